@@ -286,6 +286,107 @@ int  ptmi_model_read_weights(ptmi_model_t *m, void *blob, size_t bytes);
  * pt_train.c:342-370) of the last train step to host memory.           */
 int  ptmi_model_read_grads(ptmi_model_t *m, float *out, size_t n_floats);
 
+/* ── many requests over one paged cache (device pointers) ─────────────
+ * The operators of a server's step: bookkeeping, cache write, attention,
+ * choice of the next tokens.  No counterpart in the reference, which runs
+ * one sequence with a cache of its own (pitorch/model/llama2.h:46-47) and
+ * samples on the host (pitorch/text/pt_text.c:209-308).
+ *
+ * Keys and values of every request live in pages of page_size positions,
+ * handed out from one pool.  Row s of the block table [n_requests]
+ * [table_width] names request s's pages in order: its position p is in page
+ * block_table[s][p / page_size].  The slot of a position is
+ * page * page_size + p % page_size.  New tokens of all requests stand in one
+ * array of rows, request by request: rows [row_start[s], row_start[s+1]).
+ *
+ * Lengths, tables and slots are read on the device, so a captured call
+ * serves every step.  Every call enqueues on `stream` (NULL = the library
+ * stream), allocates nothing, waits for nothing and may be captured.
+ * Arrays that a call writes must not overlap others of the call, unless it
+ * says so.  All memory belongs to the library's GPU.                    */
+enum { PTMI_F32 = 0, PTMI_BF16 = 1 };
+typedef struct {
+    void *k, *v;             /* 16-byte aligned                           */
+    int   type;              /* of their elements: PTMI_F32 or PTMI_BF16  */
+    int   n_pages, page_size, n_kv_heads, head_dim;
+    /* element i of key head h at slot (page, p) is
+     * k[page*page_stride + p*pos_stride + h*head_stride + i]: multiples of 4,
+     * at least head_dim; v alike                                         */
+    long  page_stride, pos_stride, head_stride;
+} ptmi_pages_t;
+
+/* The bookkeeping of one step: from each request's cached length past[s]
+ * and its new tokens fresh[s] (0: none this time; -1: the request has ended)
+ * its length kv_len[s] = past + fresh (0 when ended), row_start[0..
+ * n_requests], and for every row its position and its slot.  Pages that
+ * positions need for the first time come off the pool, a stack of page
+ * numbers pool[0..*pool_count), room for n_pages of them; pages of ended
+ * requests first go onto it (both in the order of requests, then of pages).
+ * *pool_left gets the new count.  Rows from row_start[n_requests] on get
+ * position and slot -1.  kv_len may be past, and pool_left pool_count.
+ * *status = 0, or the sum of 1: pool short, 2: a request needs more than
+ * table_width pages, 4: more than max_rows rows, 8: a bad length, count or
+ * page number.  Then the step is refused as a whole: lengths, tables and
+ * pool stay as they are and there are no rows (row_start is all 0).      */
+int ptmi_paged_plan_dev(const int *past, const int *fresh, int n_requests, int *pool, const int *pool_count,
+                        int n_pages, int page_size, int *block_table, int table_width, int *kv_len,
+                        int *pool_left, int *row_start, int *row_pos, int *row_slot, int max_rows, int *status,
+                        void *stream);
+
+/* One layer's new keys and values go to their slots, and RoPE to q and k on
+ * the way.  Row r has n_heads query heads at q + r*ldq and the cache's key
+ * and value heads at k and v + r*ldkv.  rope: [rope_len][head_dim/2][2]
+ * (cos, sin) of every position, for the pairs (2i, 2i+1); NULL: q and k as
+ * they are (row_pos is then not read).  Rotated queries go to q_out + r*ldo,
+ * which may be q; q NULL: keys and values only.  Rows whose slot lies
+ * outside the cache, or whose position lies outside rope, are skipped.
+ * bf16 pages get values rounded to nearest even.  Two rows of one slot
+ * leave either's there.                                                  */
+int ptmi_paged_store_dev(const ptmi_pages_t *pages, const float *q, long ldq, float *q_out, long ldo, int n_heads,
+                         const float *k, const float *v, long ldkv, const int *row_pos, const int *row_slot,
+                         int rows, const float *rope, int rope_len, void *stream);
+
+/* Attention of the new rows over the paged cache (which holds them already).
+ * Row i of request s's n = row_start[s+1] - row_start[s] rows stands at
+ * position p = kv_len[s] - n + i and sees positions 0..p:
+ *   out = sum_j softmax_j(scale * q.k_j) v_j
+ * for each of n_heads heads, head h with key head h / (n_heads/n_kv_heads).
+ * head_dim: a multiple of 4, at most 128.  q and out rows: [n_heads]
+ * [head_dim], row strides multiples of 4 floats, 16-byte aligned.  Positions
+ * in pages outside [0, n_pages) count as unseen; a row that sees nothing gets
+ * zeros; rows outside every request, or from `rows` on, are left as they are.
+ * Sums are held in fp32, each score and output within a few roundings of
+ * fp32.  A query or key that is not finite makes NaN of the heads of the
+ * rows that see it (a key that an infinity gives the score -infinity may
+ * count as unseen), a value that is not finite makes its element of them
+ * not finite; other rows and heads are not touched.
+ * max_new: the most rows any one request has (0: not known); one that has
+ * more may be left as it is.  work: ptmi_paged_attention_work bytes, 16-byte
+ * aligned, whatever they hold; calls that can overlap need their own.     */
+int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, int table_width,
+                             const int *row_start, const int *kv_len, int n_requests, int max_new, const float *q,
+                             long ldq, float *out, long ldo, int rows, int n_heads, float scale, void *work,
+                             size_t work_bytes, void *stream);
+/* The bytes it needs, for any lengths; 0 and an error for arguments that
+ * ptmi_paged_attention_dev refuses.                                       */
+size_t ptmi_paged_attention_work(const ptmi_pages_t *pages, int n_heads, int max_new);
+
+/* One token per row of logits [rows][vocab] (row stride ld), by the row's own
+ * parameters; a NULL array switches its parameter off.  With the logits l in
+ * descending order, ties by index, and w = e^((l - max)/temperature):
+ *   top_k > 0: the first top_k stay;
+ *   min_p:     of these, those with w >= min_p (at least the first);
+ *   top_p < 1: of these, the shortest beginning whose sum reaches top_p of
+ *              theirs (at least the first).
+ * The token is the first index at which the sum of what stayed, taken in the
+ * order of indices, exceeds u times its whole (u clamped to [0, 1)).
+ * temperature <= 0 (or NaN): the first index of the maximum.  NaN logits
+ * count as -infinity, and with nothing above that the token is -1; among
+ * infinite maxima only they stay.  w below 2^-45 counts as 0.  Sums are
+ * integers of 2^-44: a row's result depends on nothing else.             */
+int ptmi_sample_dev(const float *logits, long ld, int rows, int vocab, const float *temperature, const int *top_k,
+                    const float *top_p, const float *min_p, const float *u, int *token, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

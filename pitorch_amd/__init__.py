@@ -9,8 +9,11 @@ This package only binds them with ctypes for tests and the benchmark.  There
 is no CPU fallback: if the libraries are missing, loading raises.
 """
 from ._ffi import (  # noqa: F401
-    PtmiError,
+    BF16,
+    F32,
     Model,
+    Pages,
+    PtmiError,
     decode_step_plan,
     gemm_plan,
     lib_dir,

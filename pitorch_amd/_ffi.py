@@ -16,6 +16,16 @@ class Span(ctypes.Structure):
                 ("depth", ctypes.c_int), ("start_us", ctypes.c_double), ("dur_us", ctypes.c_double)]
 
 
+class Pages(ctypes.Structure):
+    """ptmi_pages_t (include/ptmi.h)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("type", ctypes.c_int), ("n_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("page_stride", ctypes.c_long),
+                ("pos_stride", ctypes.c_long), ("head_stride", ctypes.c_long)]
+
+
+F32, BF16 = 0, 1    # ptmi_pages_t.type
+
+
 def lib_dir():
     return os.path.join(_HERE, "lib")
 
@@ -92,6 +102,12 @@ def load_ptmi():
          [_vp, _c_int_p, i, f, _c_float_p, ctypes.POINTER(Span), i, ctypes.POINTER(i)])
     _sig(L, "ptmi_model_read_weights", i, [_vp, _vp, sz])
     _sig(L, "ptmi_model_read_grads", i, [_vp, _c_float_p, sz])
+    lg, pages = ctypes.c_long, ctypes.POINTER(Pages)
+    _sig(L, "ptmi_paged_plan_dev", i, [_vp, _vp, i, _vp, _vp, i, i, _vp, i, _vp, _vp, _vp, _vp, _vp, i, _vp, _vp])
+    _sig(L, "ptmi_paged_store_dev", i, [pages, _vp, lg, _vp, lg, i, _vp, _vp, lg, _vp, _vp, i, _vp, i, _vp])
+    _sig(L, "ptmi_paged_attention_dev", i, [pages, _vp, i, _vp, _vp, i, i, _vp, lg, _vp, lg, i, i, f, _vp, sz, _vp])
+    _sig(L, "ptmi_paged_attention_work", sz, [pages, i, i])
+    _sig(L, "ptmi_sample_dev", i, [_vp, lg, i, i, _vp, _vp, _vp, _vp, _vp, _vp, _vp])
     _ptmi = L
     return L
 
