@@ -351,8 +351,9 @@ int ptmi_paged_store_dev(const ptmi_pages_t *pages, const float *q, long ldq, fl
  * position p = kv_len[s] - n + i and sees positions 0..p:
  *   out = sum_j softmax_j(scale * q.k_j) v_j
  * for each of n_heads heads, head h with key head h / (n_heads/n_kv_heads).
- * head_dim: a multiple of 4, at most 128.  q and out rows: [n_heads]
- * [head_dim], row strides multiples of 4 floats, 16-byte aligned.  Positions
+ * At most 128 heads share a key head; head_dim: a multiple of 4, at most 128.
+ * q and out rows: [n_heads][head_dim], row strides multiples of 4 floats,
+ * 16-byte aligned; table_width * page_size under 2^31 - 4096.  Positions
  * in pages outside [0, n_pages) count as unseen; a row that sees nothing gets
  * zeros; rows outside every request, or from `rows` on, are left as they are.
  * Sums are held in fp32, each score and output within a few roundings of

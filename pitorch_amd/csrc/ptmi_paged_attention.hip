@@ -1,8 +1,20 @@
 // Attention of new rows over a paged cache.
 //
-// One wave per row and head takes 64 keys at a time, one per lane, with a
-// running maximum m and sum l of the softmax:
-//   m' = max(m, s), l' = l e^(m - m') + sum e^(s - m'), o' = o e^(m - m') + sum e^(s - m') v.
+// For one key head of one request, M = new tokens x query heads that share
+// it are the rows of two products over the keys, joined by a softmax that
+// runs along with them (running maximum m, sum l, weighted values o):
+//   m' = max(m, s), l' = l 2^(m - m') + sum 2^(s - m'), o' = o 2^(m - m') + sum 2^(s - m') v
+// with scores s = (scale log2(e) q).k, so that every e^x is one 2^x.
+//
+// Two kernels, by M.  Up to 16 rows (single tokens, a few tokens) are bound
+// by the bytes of the cache: k_attn_few streams them through the fp32 matrix
+// instructions.  More rows are bound by the products: k_attn_tile.
+//
+// Lengths are known on the device alone, so the launch does not depend on
+// them: the work of all requests is one axis of units of 64 keys (request by
+// request, head by head, tile of rows by tile), and every workgroup takes an
+// equal stretch of it.  A stretch that ends inside a head leaves its part
+// (m, l, o) in the workspace, and k_attn_join adds such parts up in order.
 #include "ptmi_paged.h"
 
 #include <climits>
@@ -11,6 +23,18 @@
 namespace ptmi {
 
 namespace {
+
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h4v __attribute__((ext_vector_type(4)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f2v __attribute__((ext_vector_type(2)));
+
+constexpr int kUnit = 64;            // keys of a unit
+constexpr int kFewRows = 16;         // rows of k_attn_few
+constexpr int kTileRows = 128;       // rows of a tile of k_attn_tile
+constexpr int kThreads = 256;
 
 struct AttnArgs {
     const void *k, *v;
@@ -21,87 +45,879 @@ struct AttnArgs {
     const int *row_start, *kv_len; int n_req;
     const float *q; long ldq;
     float *out; long ldo;
-    int rows, heads, kv_heads, hd;
-    float scale;
+    int rows, kv_heads, hd;
+    FastDiv group;                   // query heads of a key head
+    int tile_tokens;                 // tokens of a tile: whole tokens of at most kTileRows rows
+    float qscale;                    // scale * log2(e)
+    float *parts;                    // parts of heads cut between workgroups
 };
 
-template <bool BF16>
-__device__ __forceinline__ float4 get4(const void *base, long at) {
-    if constexpr (BF16) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const unsigned short *>(base) + at);
-        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
-                           __uint_as_float(w.y & 0xFFFF0000u));
-    } else {
-        return *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
+// ── the axis of units ────────────────────────────────────────────────────
+struct Request { int n, row0, len; };
+
+__device__ __forceinline__ Request request(const AttnArgs &a, int s) {
+    Request r;
+    r.row0 = a.row_start[s];
+    r.n = min(max(a.row_start[s + 1] - r.row0, 0), a.rows);
+    r.len = (int)min((long)max(a.kv_len[s], 0), (long)a.width * a.page.d);
+    return r;
+}
+
+// sum_{i<n} floor((a i + b) / 64)
+__device__ long floor_sum(unsigned n, unsigned a, unsigned b) {
+    long sum = 0;
+    unsigned m = kUnit;
+    for (;;) {
+        sum += (long)n * (n - 1) / 2 * (a / m) + (long)n * (b / m);
+        a %= m;
+        b %= m;
+        const unsigned long y = (unsigned long)a * n + b;
+        if (y < m) return sum;
+        n = (unsigned)(y / m);
+        b = (unsigned)(y % m);
+        const unsigned t = m;
+        m = a;
+        a = t;
     }
 }
 
-template <bool BF16>
-__global__ __launch_bounds__(64) void k_attn_simple(AttnArgs a) {
-    __shared__ float qs[128], ps[64];
-    __shared__ long at[64];
-    const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    // the request whose rows hold r
-    int lo = 0, hi = a.n_req;                               // row_start[lo] <= r < row_start[hi]
-    if (r < a.row_start[0] || r >= a.row_start[a.n_req]) return;
+// Units of one key head of a request; 0: the other kernel's.  A tile of
+// rows counts the keys its last whole token would see: at most a unit or
+// two too many at the request's end, which find no key and cost nothing.
+__device__ __forceinline__ unsigned tile_keys0(const AttnArgs &a, const Request &r) {
+    return (unsigned)max(r.len - r.n, 0) + a.tile_tokens + kUnit - 1;
+}
+template <bool TILE>
+__device__ __forceinline__ long head_units(const AttnArgs &a, const Request &r) {
+    const bool few = (long)r.n * a.group.d <= kFewRows;
+    if (r.n == 0 || few == TILE) return 0;
+    if constexpr (TILE)
+        return floor_sum((r.n + a.tile_tokens - 1) / a.tile_tokens, a.tile_tokens, tile_keys0(a, r));
+    else
+        return max(1, (r.len + kUnit - 1) / kUnit);
+}
+
+// The units of 256 requests at a time, as sums in shared memory.
+struct Axis {
+    long pre[kThreads + 1];          // units before request c0 + i
+    long total;                      // of all requests
+    int c0;
+};
+
+__device__ __forceinline__ long wave_scan(long v) {        // inclusive
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+// Fills x for requests [c0, c0 + 256) after `before` units; every thread takes part.
+template <bool TILE>
+__device__ void axis_fill(const AttnArgs &a, Axis &x, int c0, long before) {
+    __shared__ long wsum[kThreads / 64];
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+    long v = 0;
+    if (c0 + t < a.n_req) v = head_units<TILE>(a, request(a, c0 + t)) * a.kv_heads;
+    const long incl = wave_scan(v);
+    __syncthreads();
+    if (lane == 63) wsum[w] = incl;
+    __syncthreads();
+    for (int i = 0; i < w; i++) before += wsum[i];
+    x.pre[t + 1] = before + incl;
+    if (t == 0) { x.pre[0] = before; x.c0 = c0; }
+    __syncthreads();
+}
+
+// Counts all units; x then holds the requests' first 256.
+template <bool TILE>
+__device__ void axis_init(const AttnArgs &a, Axis &x) {
+    if (a.n_req > kThreads) {
+        long total = 0;
+        for (int c0 = 0; c0 < a.n_req; c0 += kThreads) {
+            axis_fill<TILE>(a, x, c0, total);
+            total = x.pre[kThreads];
+        }
+        axis_fill<TILE>(a, x, 0, 0);
+        if (threadIdx.x == 0) x.total = total;
+    } else {
+        axis_fill<TILE>(a, x, 0, 0);
+        if (threadIdx.x == 0) x.total = x.pre[kThreads];
+    }
+    __syncthreads();
+}
+
+// The request that holds unit u < total (refills x as needed).
+template <bool TILE>
+__device__ int axis_find(const AttnArgs &a, Axis &x, long u) {
+    while (u >= x.pre[kThreads]) axis_fill<TILE>(a, x, x.c0 + kThreads, x.pre[kThreads]);
+    while (u < x.pre[0]) axis_fill<TILE>(a, x, 0, 0);       // (only ever walked forward)
+    int lo = 0, hi = kThreads;                              // pre[lo] <= u < pre[hi]
     while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.row_start[mid] <= r) lo = mid;
+        const int mid = (lo + hi) >> 1;
+        if (x.pre[mid] <= u) lo = mid;
         else hi = mid;
     }
-    const int n = a.row_start[lo + 1] - a.row_start[lo];
-    const int len = min(max(a.kv_len[lo], 0), (int)min((long)a.width * a.page.d, (long)INT_MAX));
-    const int keys = min(len, len - n + (r - a.row_start[lo]) + 1);
-    const int kvh = h / (a.heads / a.kv_heads);
-    for (int d = lane; d < a.hd; d += 64) qs[d] = a.q[r * a.ldq + (long)h * a.hd + d];
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int k0 = 0; k0 < keys; k0 += 64) {
-        const int key = k0 + lane;
-        float s = -INFINITY;
-        long off = -1;
-        if (key < keys) {
-            const int j = a.page.quot(key), pg = a.table[(long)lo * a.width + j];
-            if ((unsigned)pg < (unsigned)a.n_pages) {
-                off = pg * a.page_stride + (long)(key - j * a.page.d) * a.pos_stride + kvh * a.head_stride;
-                s = 0.0f;
-                for (int d = 0; d < a.hd; d += 4) {
-                    const float4 x = get4<BF16>(a.k, off + d);
-                    s = fmaf(x.x, qs[d], s); s = fmaf(x.y, qs[d + 1], s);
-                    s = fmaf(x.z, qs[d + 2], s); s = fmaf(x.w, qs[d + 3], s);
+    return x.c0 + lo;
+}
+
+// The stretches: workgroup g of n takes units [first(g), first(g + 1)).
+struct Split {
+    long each, more;                 // the first `more` take each + 1
+    __device__ Split(long total, int n) {
+        each = total < INT_MAX ? (long)((unsigned)total / (unsigned)n) : total / n;
+        more = total - each * n;
+    }
+    __device__ long first(int g) const { return g * each + min((long)g, more); }
+};
+
+// One item of the axis: a head's keys for one tile of rows, units [a, b).
+struct Item {
+    int s, kvh, tile;
+    long a, b;
+    Request r;
+};
+template <bool TILE>
+__device__ Item axis_item(const AttnArgs &a, Axis &x, long u) {
+    Item it;
+    it.s = axis_find<TILE>(a, x, u);
+    it.r = request(a, it.s);
+    const long per = head_units<TILE>(a, it.r), base = x.pre[it.s - x.c0];
+    it.kvh = (int)((u - base) / per);
+    it.a = base + it.kvh * per;
+    it.b = it.a + per;
+    it.tile = 0;
+    if constexpr (TILE) {
+        const unsigned tt = a.tile_tokens, b0 = tile_keys0(a, it.r);
+        unsigned lo = 0, hi = (it.r.n + tt - 1) / tt;       // sum(lo) <= u - a < sum(hi)
+        while (hi - lo > 1) {
+            const unsigned mid = (lo + hi) >> 1;
+            if (floor_sum(mid, tt, b0) <= u - it.a) lo = mid;
+            else hi = mid;
+        }
+        it.tile = (int)lo;
+        it.a += floor_sum(lo, tt, b0);
+        it.b = it.a + (long)((b0 + lo * tt) / kUnit);
+    }
+    return it;
+}
+
+// XCD x runs every eighth workgroup: give each XCD neighbouring stretches,
+// so that the tiles of one head find its keys in that XCD's L2.
+__device__ __forceinline__ int stretch_of_block() {
+    const int n = gridDim.x, b = blockIdx.x;               // (n a multiple of 8)
+    return (b & 7) * (n >> 3) + (b >> 3);
+}
+
+// ── loads ────────────────────────────────────────────────────────────────
+template <bool BF16> struct Raw4 { float4 x; };
+template <> struct Raw4<true> { uint2 x; };
+
+template <bool BF16>
+__device__ __forceinline__ Raw4<BF16> raw_load(const void *base, long at) {
+    Raw4<BF16> r;
+    if constexpr (BF16) r.x = *reinterpret_cast<const uint2 *>(static_cast<const unsigned short *>(base) + at);
+    else r.x = *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ Raw4<BF16> raw_zero() {
+    Raw4<BF16> r;
+    if constexpr (BF16) r.x = make_uint2(0, 0);
+    else r.x = make_float4(0.f, 0.f, 0.f, 0.f);
+    return r;
+}
+__device__ __forceinline__ f4v widen(const Raw4<false> &r) { return f4v{r.x.x, r.x.y, r.x.z, r.x.w}; }
+__device__ __forceinline__ f4v widen(const Raw4<true> &r) {
+    return f4v{__uint_as_float(r.x.x << 16), __uint_as_float(r.x.x & 0xFFFF0000u), __uint_as_float(r.x.y << 16),
+               __uint_as_float(r.x.y & 0xFFFF0000u)};
+}
+
+// Element offset of a key's position from its page number; -1: not there.
+__device__ __forceinline__ long key_offset(const AttnArgs &a, int key, int limit, int pg, int kvh) {
+    if (key >= limit || (unsigned)pg >= (unsigned)a.n_pages) return -1;
+    return pg * a.page_stride + (long)(key - a.page.quot(key) * a.page.d) * a.pos_stride + kvh * a.head_stride;
+}
+__device__ __forceinline__ int page_of(const AttnArgs &a, int s, int key, int limit) {
+    return key < limit ? a.table[(long)s * a.width + a.page.quot(key)] : -1;
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+
+// ── few rows ─────────────────────────────────────────────────────────────
+// v_mfma_f32_16x16x4_f32: lane l supplies A[l%16][l/16] and B[l/16][l%16];
+// result register r of lane l is C[4*(l/16) + r][l%16].  S^T = K.Q^T: a
+// lane's four scores are keys 4g..4g+3 of row l%16, the operands of
+// O^T += V^T.P^T as they stand.  The contraction over head_dim may take its
+// index in any order that q and k share (lane group g takes float4s g, g+4,
+// ...), and the rows of V^T too: lane li loads float4s li, li+16 of a value
+// row, whose component e is row li of result tile e.  So K and V both come as
+// 16-byte loads of whole rows.
+__device__ __forceinline__ f4v mfma4(float a, float b, f4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// Floats of a part: o [16][pitch], then (m, l) [16].
+constexpr int few_pitch(int hq) { return hq > 4 ? 128 : 64; }
+constexpr int few_part(int hq) { return kFewRows * few_pitch(hq) + 2 * kFewRows; }
+
+template <int HQ, bool PAD, bool BF16>
+struct FewBlock {                    // 16 keys of one head
+    Raw4<BF16> k[HQ], v[4][HQ > 4 ? 2 : 1];
+    long off;                        // lane's key li; -1: not there
+};
+
+template <int HQ, bool PAD, bool BF16>
+__device__ __forceinline__ void few_load(const AttnArgs &a, FewBlock<HQ, PAD, BF16> &b, int n4) {
+    constexpr int C4 = HQ > 4 ? 2 : 1;
+    const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < HQ; j++) {
+        const int i = 4 * j + g;
+        b.k[j] = raw_zero<BF16>();
+        if (b.off >= 0 && (!PAD || i < n4)) b.k[j] = raw_load<BF16>(a.k, b.off + 4 * i);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+        const long off = __shfl(b.off, 4 * g + s);
+#pragma unroll
+        for (int c = 0; c < C4; c++) {
+            const int i = li + 16 * c;
+            b.v[s][c] = raw_zero<BF16>();
+            if (off >= 0 && (!PAD || i < n4)) b.v[s][c] = raw_load<BF16>(a.v, off + 4 * i);
+        }
+    }
+}
+
+template <int HQ, bool PAD, bool BF16>
+__global__ __launch_bounds__(kThreads) void k_attn_few(AttnArgs a) {
+    constexpr int C4 = HQ > 4 ? 2 : 1, NC = 4 * C4, PITCH = few_pitch(HQ) + 4, NW = kThreads / 64;
+    __shared__ Axis axis;
+    __shared__ __align__(16) float red[NW * kFewRows * PITCH];
+    __shared__ float st_m[NW][kFewRows], st_l[NW][kFewRows];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+    const int hd = PAD ? a.hd : 16 * HQ, n4 = hd >> 2, G = a.group.d;
+    axis_init<false>(a, axis);
+    const Split split(axis.total, gridDim.x);
+    const int wg = stretch_of_block();
+    const long u1 = split.first(wg + 1);
+    for (long u = split.first(wg); u < u1;) {
+        const Item it = axis_item<false>(a, axis, u);
+        const long ue = min(u1, it.b);
+        const int M = it.r.n * G, len = it.r.len;
+        // this lane's row: token li / G, query head li % G
+        const int tok = a.group.quot(li), row = it.r.row0 + tok;
+        const bool live = li < M && (unsigned)row < (unsigned)a.rows;
+        const float *qrow = a.q + row * a.ldq + (long)(it.kvh * G + li - tok * G) * hd;
+        f4v qf[HQ];
+#pragma unroll
+        for (int j = 0; j < HQ; j++) {
+            const int i = 4 * j + g;
+            qf[j] = f4v{0.f, 0.f, 0.f, 0.f};
+            if (live && (!PAD || i < n4)) qf[j] = *reinterpret_cast<const f4v *>(qrow + 4 * i) * a.qscale;
+        }
+        const int see = len - it.r.n + tok + 1;             // keys [0, see)
+        const int see0 = len - it.r.n + 1;                  // of the first row
+        f4v acc[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) acc[c] = f4v{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.0f;
+        // this wave's 16 keys of every unit; two blocks of keys and one more of page numbers in flight
+        int kb = (int)(u - it.a) * 4 + wave;
+        const int kend = (int)(ue - it.a) * 4;
+        FewBlock<HQ, PAD, BF16> cur, nxt;
+        cur.off = key_offset(a, kb * 16 + li, len, page_of(a, it.s, kb * 16 + li, len), it.kvh);
+        int pg = page_of(a, it.s, (kb + NW) * 16 + li, len);
+        few_load(a, cur, n4);
+        for (; kb < kend; kb += NW) {
+            nxt.off = kb + NW < kend ? key_offset(a, (kb + NW) * 16 + li, len, pg, it.kvh) : -1;
+            few_load(a, nxt, n4);
+            pg = page_of(a, it.s, (kb + 2 * NW) * 16 + li, len);
+            f4v s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+            for (int j = 0; j < HQ; j++) {
+                const f4v x = widen(cur.k[j]);
+                s0 = mfma4(x.x, qf[j].x, s0);
+                s1 = mfma4(x.y, qf[j].y, s1);
+                s0 = mfma4(x.z, qf[j].z, s0);
+                s1 = mfma4(x.w, qf[j].w, s1);
+            }
+            const f4v s = s0 + s1;
+            const unsigned there = (unsigned)__ballot(cur.off >= 0) >> (4 * g);   // bit r: key 4g + r
+            const int key = kb * 16 + 4 * g;
+            bool use[4];
+            float bm = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                use[r] = (there >> r & 1) && key + r < see;
+                bm = use[r] ? fmaxf(bm, s[r]) : bm;
+            }
+            LanePair pr = pl16(bm);
+            bm = fmaxf(pr.lo, pr.hi);
+            pr = pl32(bm);
+            const float mn = fmaxf(m, fmaxf(pr.lo, pr.hi)), ref = mn == -INFINITY ? 0.0f : mn;
+            if (__any(mn > m)) {
+                const float f = exp2_hw(m - ref);
+                l *= f;
+                m = mn;
+#pragma unroll
+                for (int c = 0; c < NC; c++) acc[c] *= f;
+            }
+            float p[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float e = exp2_hw(s[r] - ref);
+                p[r] = use[r] ? e : 0.0f;
+                l += p[r];
+            }
+            f4v v[4][C4];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int c = 0; c < C4; c++) v[t][c] = widen(cur.v[t][c]);
+            if (kb * 16 + 16 > see0) {
+                // rows that do not see a key must not meet its value if that is not finite (0 * NaN):
+                // it leaves the product, and the rows that see it get a NaN in its place
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int c = 0; c < C4; c++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const unsigned long bad = __ballot(!finite_bits(v[t][c][e]));
+                            if (!bad) continue;
+                            if (!finite_bits(v[t][c][e])) v[t][c][e] = 0.0f;
+#pragma unroll
+                            for (int h = 0; h < 4; h++)
+#pragma unroll
+                                for (int r = 0; r < 4; r++)
+                                    if ((bad >> (16 * h + 4 * g + r) & 1) && kb * 16 + 4 * h + t < see)
+                                        acc[4 * c + e][r] = NAN;
+                        }
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int c = 0; c < NC; c++) acc[c] = mfma4(v[t][c >> 2][c & 3], p[t], acc[c]);
+            cur = nxt;
+        }
+        // the four waves' sums, one maximum for all
+        l = xsum32(xsum16(l));
+        if (g == 0) { st_m[wave][li] = m; st_l[wave][li] = l; }
+        __syncthreads();
+        float gm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NW; w++) gm = fmaxf(gm, st_m[w][li]);
+        const float ref = gm == -INFINITY ? 0.0f : gm, f = exp2_hw(m - ref);
+        if (li < M) {
+#pragma unroll
+            for (int c = 0; c < C4; c++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const f4v o = {acc[4 * c][r], acc[4 * c + 1][r], acc[4 * c + 2][r], acc[4 * c + 3][r]};
+                    *reinterpret_cast<f4v *>(red + (wave * kFewRows + li) * PITCH + 4 * (16 * c + 4 * g + r)) = o * f;
                 }
-                s *= a.scale;
+        }
+        __syncthreads();
+        const bool whole = u == it.a && ue == it.b;
+        float *part = a.parts + (long)(2 * wg + (u == it.a)) * few_part(HQ);
+        for (int e = threadIdx.x; e < M * n4; e += kThreads) {
+            const int i = e / n4, c = e - i * n4;
+            f4v o = *reinterpret_cast<const f4v *>(red + i * PITCH + 4 * c);
+#pragma unroll
+            for (int w = 1; w < NW; w++) o += *reinterpret_cast<const f4v *>(red + (w * kFewRows + i) * PITCH + 4 * c);
+            float im = -INFINITY, il = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; w++) im = fmaxf(im, st_m[w][i]);
+            const float iref = im == -INFINITY ? 0.0f : im;
+#pragma unroll
+            for (int w = 0; w < NW; w++) il += st_l[w][i] * exp2_hw(st_m[w][i] - iref);
+            if (whole) {
+                const int t = a.group.quot(i), r = it.r.row0 + t;
+                if ((unsigned)r < (unsigned)a.rows)
+                    *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(it.kvh * G + i - t * G) * hd + 4 * c) =
+                        o * (il == 0.0f ? 0.0f : 1.0f / il);
+            } else {
+                *reinterpret_cast<f4v *>(part + i * few_pitch(HQ) + 4 * c) = o;
+                if (c == 0) {
+                    part[kFewRows * few_pitch(HQ) + 2 * i] = im;
+                    part[kFewRows * few_pitch(HQ) + 2 * i + 1] = il;
+                }
             }
         }
-        const float mn = fmaxf(m, group_max<64>(s)), ref = mn == -INFINITY ? 0.0f : mn;
-        const float f = expf(m - ref), p = expf(s - ref);
-        l = l * f + group_sum<64>(p);
+        __syncthreads();
+        u = ue;
+    }
+}
+
+// Joins the parts of heads that workgroup boundaries cut: block g takes the
+// head that boundary g cuts, if no earlier boundary does.
+template <int HQ>
+__global__ __launch_bounds__(kThreads) void k_attn_few_join(AttnArgs a, int n_wg) {
+    __shared__ Axis axis;
+    const int g = (int)blockIdx.x + 1, hd = a.hd, n4 = hd >> 2, G = a.group.d;
+    axis_init<false>(a, axis);
+    const Split split(axis.total, n_wg);
+    const long u = split.first(g);
+    if (u >= axis.total || u == 0) return;
+    const Item it = axis_item<false>(a, axis, u);
+    if (it.a >= u || split.first(g - 1) > it.a) return;
+    const int M = it.r.n * G;
+    int last = g;                                           // the workgroup of the head's last unit
+    while (split.first(last + 1) < it.b) last++;
+    auto part_of = [&](int w) { return a.parts + (long)(2 * w + (w == g - 1)) * few_part(HQ); };
+    for (int e = threadIdx.x + blockIdx.y * kThreads; e < M * n4; e += kThreads * gridDim.y) {
+        const int i = e / n4, c = e - i * n4;
+        float m = -INFINITY, l = 0.0f;
+        f4v o = {0.f, 0.f, 0.f, 0.f};
+        for (int w = g - 1; w <= last; w++) {
+            const float *p = part_of(w);
+            const float pm = p[kFewRows * few_pitch(HQ) + 2 * i], pl = p[kFewRows * few_pitch(HQ) + 2 * i + 1];
+            const f4v po = *reinterpret_cast<const f4v *>(p + i * few_pitch(HQ) + 4 * c);
+            const float mn = fmaxf(m, pm), ref = mn == -INFINITY ? 0.0f : mn;
+            const float f = exp2_hw(m - ref), pf = exp2_hw(pm - ref);
+            l = l * f + pl * pf;
+            o = o * f + po * pf;
+            m = mn;
+        }
+        const int t = a.group.quot(i), r = it.r.row0 + t;
+        if ((unsigned)r < (unsigned)a.rows)
+            *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(it.kvh * G + i - t * G) * hd + 4 * c) =
+                o * (l == 0.0f ? 0.0f : 1.0f / l);
+    }
+}
+
+// ── many rows ────────────────────────────────────────────────────────────
+// fp32 products on the 16-bit matrix cores: x = 2^e (h + l) with h the
+// nearest fp16 of x 2^-e and l that of the rest, 22 bits of x; of the four
+// products of two such numbers l.l, under 2^-22 of the whole, is left out.
+// e is the tile's (a row of q's) largest exponent less kTop, so h and l keep
+// all their bits down to 2^-16 of the largest value, and below that an error
+// of 2^-39 of it.  Three v_mfma_f32_32x32x16_f16 per product run at a third of
+// 1180 TFLOP/s (what a large fp16 product reaches here), the fp32 matrix
+// instructions at 154.  bf16 keys and values are h alone: two products.
+//
+// Wave w holds rows 32w.. of the tile as columns: S^T = K.Q^T leaves a lane
+// with 32 of the unit's scores of its row l%32 and its partner l^32 with the
+// others; its result registers, split, are the operand of O^T += V^T.P^T, if
+// V^T's columns (keys) stand in the same order: registers 4b..4b+3 of half h
+// are keys 8b + 4h.. of a 32-key block.
+constexpr int kTop = 14;             // largest |h| < 2^15
+constexpr int kBias = 9;             // weights are held times 2^9:
+constexpr float kLazy = 6.0f;        // a maximum up to 2^6 above m does not move m (2^15 < 65504)
+
+constexpr int tile_part(int dt) { return kTileRows * (32 * dt + 2); }    // floats
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(min(max(e, -126), 127) + 127) << 23); }
+
+__device__ __forceinline__ f16v mfma16(h8v a, h8v b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ h2v cvt2(float x, float y) {
+    const f2v v = {x, y};
+    return __builtin_convertvector(v, h2v);
+}
+__device__ __forceinline__ h2v rest2(float x, float y, h2v h) {
+    return cvt2(fmaf((float)h.x, -1.0f, x), fmaf((float)h.y, -1.0f, y));
+}
+
+template <int DT, bool BF16>
+struct TileLds {
+    static constexpr int HP = 32 * DT, KP = HP + 8, VP = kUnit + 8;      // pitches in halves
+    static constexpr int PL = BF16 ? 1 : 2;                              // planes: h, l
+    _Float16 k[PL][kUnit * KP], v[PL][HP * VP];
+    long off[4][kUnit];              // units u..u+3: offsets of their keys, -1: not there
+    int all[4];                      // whether all 64 are
+    unsigned kmax[2][4], vmax[2][4];
+};
+
+template <int DT, bool BF16>
+__global__ __launch_bounds__(kThreads, DT <= 2 ? 2 : 1) void k_attn_tile(AttnArgs a) {
+    typedef TileLds<DT, BF16> Lds;
+    constexpr int HP = Lds::HP, KP = Lds::KP, VP = Lds::VP, PL = Lds::PL, KS = HP / 16;
+    constexpr int VT = (128 * DT + kThreads - 1) / kThreads;             // value tasks of a thread: 4 keys x 4 columns
+    __shared__ Axis axis;
+    __shared__ __align__(16) Lds lds;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+    const int hd = a.hd, n4 = hd >> 2, G = a.group.d;
+    axis_init<true>(a, axis);
+    const Split split(axis.total, gridDim.x);
+    const int wg = stretch_of_block();
+    const long u1 = split.first(wg + 1);
+    for (long u = split.first(wg); u < u1;) {
+        const Item it = axis_item<true>(a, axis, u);
+        const long ue = min(u1, it.b);
+        const int tt = a.tile_tokens, t0 = it.tile * tt;
+        const int end = min(max(it.r.len - it.r.n + min(it.r.n, t0 + tt), 0), it.r.len);   // keys the tile sees
+        // this lane's row of the tile
+        const int mrow = wave * 32 + col, tok = t0 + a.group.quot(mrow), row = it.r.row0 + tok;
+        const bool live = mrow < tt * G && tok < it.r.n && (unsigned)row < (unsigned)a.rows;
+        const long head = it.kvh * G + mrow - (tok - t0) * G;
+        const int see = it.r.len - it.r.n + tok + 1;        // its keys: [0, see)
+        const int see0 = it.r.len - it.r.n + t0 + 1;        // of the tile's first row
+        // q: columns 16 ks + 8 half .. of the row, scaled, split
+        h8v qh[KS], ql[KS];
+        int qe;
+        {
+            float x[KS][8];
+            float top = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    f4v v = {0.f, 0.f, 0.f, 0.f};
+                    const int d = 16 * ks + 8 * half + 4 * j;
+                    if (live && d < hd) v = *reinterpret_cast<const f4v *>(a.q + row * a.ldq + head * hd + d) * a.qscale;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x[ks][4 * j + e] = v[e];
+                        top = finite_bits(v[e]) ? fmaxf(top, fabsf(v[e])) : top;
+                    }
+                }
+            const LanePair pr = pl32(top);
+            qe = max((int)(__float_as_uint(fmaxf(pr.lo, pr.hi)) >> 23) - 127, -100) - kTop;
+            const float sc = pow2(-qe);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float y0 = x[ks][2 * j] * sc, y1 = x[ks][2 * j + 1] * sc;
+                    const h2v h = cvt2(y0, y1), r = rest2(y0, y1, h);
+                    qh[ks][2 * j] = h.x; qh[ks][2 * j + 1] = h.y;
+                    ql[ks][2 * j] = r.x; ql[ks][2 * j + 1] = r.y;
+                }
+        }
+        f16v acc[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[d][r] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+        int ve = -1000;                                      // acc holds values times 2^-ve
+        const int b0 = (int)(u - it.a), b1 = (int)min((long)(end + kUnit - 1) / kUnit, ue - it.a);   // units of keys
+        // Offsets of unit b's keys go to slot b & 3 two units ahead of their use, page numbers one further.
+        auto put_off = [&](int b, int pg) {
+            const long off = b < b1 ? key_offset(a, b * kUnit + lane, end, pg, it.kvh) : -1;
+            lds.off[b & 3][lane] = off;
+            const bool all = __all(off >= 0);
+            if (lane == 0) lds.all[b & 3] = all;
+        };
+        auto page_at = [&](int b) { return b < b1 ? page_of(a, it.s, b * kUnit + lane, end) : -1; };
+        int pg = -1;
+        __syncthreads();                                     // the last item's readers are done
+        if (wave == 0) {
+            const int p0 = page_at(b0), p1 = page_at(b0 + 1);
+            pg = page_at(b0 + 2);
+            put_off(b0, p0);
+            put_off(b0 + 1, p1);
+        }
+        __syncthreads();
+        Raw4<BF16> rk[HP / 16], rv[VT][4];
+        auto load = [&](int b) {
+            const long *off = lds.off[b & 3];
+            const long ko = off[tid >> 2];
+#pragma unroll
+            for (int j = 0; j < HP / 16; j++) {
+                const int i = (tid & 3) + 4 * j;
+                rk[j] = raw_zero<BF16>();
+                if (ko >= 0 && i < n4) rk[j] = raw_load<BF16>(a.k, ko + 4 * i);
+            }
+#pragma unroll
+            for (int t = 0; t < VT; t++) {
+                const int task = tid + t * kThreads, quad = task / (8 * DT), c = task % (8 * DT);
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    rv[t][s] = raw_zero<BF16>();
+                    if (quad < 16 && c < n4) {
+                        const long vo = off[4 * quad + s];
+                        if (vo >= 0) rv[t][s] = raw_load<BF16>(a.v, vo + 4 * c);
+                    }
+                }
+            }
+        };
+        if (b0 < b1) load(b0);
+        for (int b = b0; b < b1; b++) {
+            // the largest exponents of the unit
+            unsigned km = 0, vm = 0;
+#pragma unroll
+            for (int j = 0; j < HP / 16; j++) {
+                const f4v x = widen(rk[j]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) km = max(km, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+            }
+#pragma unroll
+            for (int t = 0; t < VT; t++)
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const f4v x = widen(rv[t][s]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) vm = max(vm, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+                }
+            float kf = group_max<64>(__uint_as_float(km >> 1)), vf = group_max<64>(__uint_as_float(vm >> 1));
+            km = __float_as_uint(kf) << 1;                   // (halved: as floats they are finite and in order)
+            vm = __float_as_uint(vf) << 1;
+            bool odd = false;                                // some value is not finite
+            if (km >= 0x7F800000u || vm >= 0x7F800000u) {    // rare: the largest finite one
+                odd = vm >= 0x7F800000u;
+                km = vm = 0;
+                for (int j = 0; j < HP / 16; j++) {
+                    const f4v x = widen(rk[j]);
+                    for (int e = 0; e < 4; e++) if (finite_bits(x[e])) km = max(km, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+                }
+                for (int t = 0; t < VT; t++)
+                    for (int s = 0; s < 4; s++) {
+                        const f4v x = widen(rv[t][s]);
+                        for (int e = 0; e < 4; e++) if (finite_bits(x[e])) vm = max(vm, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+                    }
+                km = __float_as_uint(group_max<64>(__uint_as_float(km >> 1))) << 1;
+                vm = __float_as_uint(group_max<64>(__uint_as_float(vm >> 1))) << 1;
+            }
+            if (lane == 0) {
+                lds.kmax[b & 1][wave] = km;
+                lds.vmax[b & 1][wave] = vm | (odd ? 0x80000000u : 0u);
+            }
+            __syncthreads();                                 // also: the last unit's readers are done
+            unsigned kt = 0, vt = 0, any_odd = 0;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                kt = max(kt, lds.kmax[b & 1][w]);
+                const unsigned x = lds.vmax[b & 1][w];
+                vt = max(vt, x & 0x7FFFFFFFu);
+                any_odd |= x & 0x80000000u;
+            }
+            const int ke = max((int)(kt >> 23) - 127, -100) - kTop;
+            const int vnew = max(ve, max((int)(vt >> 23) - 127, -100) - kTop);
+            const float ks_ = pow2(-ke), vs_ = pow2(-vnew);
+#pragma unroll
+            for (int j = 0; j < HP / 16; j++) {
+                const f4v x = widen(rk[j]) * ks_;
+                const h2v h0 = cvt2(x.x, x.y), h1 = cvt2(x.z, x.w);
+                const int at = (tid >> 2) * KP + 4 * ((tid & 3) + 4 * j);
+                *reinterpret_cast<h4v *>(&lds.k[0][at]) = h4v{h0.x, h0.y, h1.x, h1.y};
+                if constexpr (PL == 2) {
+                    const h2v l0 = rest2(x.x, x.y, h0), l1 = rest2(x.z, x.w, h1);
+                    *reinterpret_cast<h4v *>(&lds.k[PL - 1][at]) = h4v{l0.x, l0.y, l1.x, l1.y};
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < VT; t++) {
+                const int task = tid + t * kThreads, quad = task / (8 * DT), c = task % (8 * DT);
+                if (quad >= 16) continue;
+                f4v x[4];
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    x[s] = widen(rv[t][s]) * vs_;
+                    if (any_odd)
+                        for (int e = 0; e < 4; e++) if (!finite_bits(x[s][e])) x[s][e] = 0.0f;
+                }
+                // quad 4 st + 2 b + h of 16 keys stands at place 4 st + 2 h + b
+                const int place = (quad & ~3) | (quad & 1) << 1 | (quad >> 1 & 1);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const h2v h0 = cvt2(x[0][e], x[1][e]), h1 = cvt2(x[2][e], x[3][e]);
+                    const int at = (4 * c + e) * VP + 4 * place;
+                    *reinterpret_cast<h4v *>(&lds.v[0][at]) = h4v{h0.x, h0.y, h1.x, h1.y};
+                    if constexpr (PL == 2) {
+                        const h2v l0 = rest2(x[0][e], x[1][e], h0), l1 = rest2(x[2][e], x[3][e], h1);
+                        *reinterpret_cast<h4v *>(&lds.v[PL - 1][at]) = h4v{l0.x, l0.y, l1.x, l1.y};
+                    }
+                }
+            }
+            if (b + 1 < b1) load(b + 1);
+            if (wave == 0) {
+                put_off(b + 2, pg);
+                pg = page_at(b + 3);
+            }
+            __syncthreads();
+            // scores
+            f16v s[2];
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int kh = 0; kh < 2; kh++) {
+                    const int at = (kh * 32 + col) * KP + 16 * ks + 8 * half;
+                    const h8v h = *reinterpret_cast<const h8v *>(&lds.k[0][at]);
+                    s[kh] = mfma16(h, qh[ks], s[kh]);
+                    s[kh] = mfma16(h, ql[ks], s[kh]);
+                    if constexpr (PL == 2)
+                        s[kh] = mfma16(*reinterpret_cast<const h8v *>(&lds.k[PL - 1][at]), qh[ks], s[kh]);
+                }
+            const float c = pow2(ke + qe);                   // scores are s * c
+            if (!lds.all[b & 3] || b * kUnit + kUnit > see0) {
+#pragma unroll
+                for (int kh = 0; kh < 2; kh++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int key = 32 * kh + 8 * (r >> 2) + 4 * half + (r & 3);
+                        if (lds.off[b & 3][key] < 0 || b * kUnit + key >= see) s[kh][r] = -INFINITY;
+                    }
+            }
+            float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+            for (int r = 1; r < 16; r++) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
+            const LanePair pr = pl32(top);
+            top = fmaxf(pr.lo, pr.hi) * c;
+            // ve only grows; the accumulated values follow it, and m
+            if (__any(top > m + kLazy) || vnew != ve) {
+                const float mn = top > m + kLazy ? top : m;
+                const float f = exp2_hw(m - (mn == -INFINITY ? 0.0f : mn));
+                l *= f;
+                m = mn;
+                const float fv = f * (vnew - ve > 126 ? 0.0f : pow2(ve - vnew));
+                ve = vnew;
+#pragma unroll
+                for (int d = 0; d < DT; d++) acc[d] *= fv;
+            }
+            const float nm = (m == -INFINITY ? 0.0f : -m) + kBias;
+            float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+            for (int kh = 0; kh < 2; kh++) {
+#pragma unroll
+                for (int st = 0; st < 2; st++) {             // 16 keys
+                    h8v ph, pl;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float p0 = exp2_hw(fmaf(s[kh][8 * st + 2 * j], c, nm));
+                        const float p1 = exp2_hw(fmaf(s[kh][8 * st + 2 * j + 1], c, nm));
+                        sum0 += p0;
+                        sum1 += p1;
+                        const h2v h = cvt2(p0, p1), r = rest2(p0, p1, h);
+                        ph[2 * j] = h.x; ph[2 * j + 1] = h.y;
+                        pl[2 * j] = r.x; pl[2 * j + 1] = r.y;
+                    }
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const int at = (32 * d + col) * VP + 4 * (8 * kh + 4 * st + 2 * half);
+                        const h8v h = *reinterpret_cast<const h8v *>(&lds.v[0][at]);
+                        acc[d] = mfma16(h, ph, acc[d]);
+                        acc[d] = mfma16(h, pl, acc[d]);
+                        if constexpr (PL == 2)
+                            acc[d] = mfma16(*reinterpret_cast<const h8v *>(&lds.v[PL - 1][at]), ph, acc[d]);
+                    }
+                }
+            }
+            l += sum0 + sum1;
+            if (any_odd) {                                   // rows that see a value that is not finite
+                for (int key = 0; key < kUnit; key++) {
+                    const long off = lds.off[b & 3][key];
+                    if (off < 0 || b * kUnit + key >= see) continue;
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const int at = 32 * d + 8 * (r >> 2) + 4 * half;
+                            if (at < hd && !finite_bits(widen(raw_load<BF16>(a.v, off + at))[r & 3])) acc[d][r] = NAN;
+                        }
+                }
+            }
+        }
+        {
+            const LanePair pr = pl32(l);
+            l = (pr.lo + pr.hi) * pow2(-kBias);
+        }
+        const float unit = pow2(ve) * pow2(-kBias);          // what acc counts in
+        if (u == it.a && ue == it.b) {
+            if (live) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                float *o = a.out + row * a.ldo + head * hd;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        const int at = 32 * d + 8 * b + 4 * half;
+                        const f4v x = {acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]};
+                        if (at < hd) *reinterpret_cast<f4v *>(o + at) = x * unit * inv;
+                    }
+            }
+        } else {
+            // [wave][4 d + b][lane] of float4, then (m, l) [wave][lane]
+            float *part = a.parts + (long)(2 * wg + (u == it.a)) * tile_part(DT);
+            f4v *po = reinterpret_cast<f4v *>(part) + (long)wave * 4 * DT * 64 + lane;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+                    po[(4 * d + b) * 64] = f4v{acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]} * unit;
+            if (half == 0)
+                *reinterpret_cast<f2v *>(part + kTileRows * 32 * DT + 2 * mrow) = f2v{m, l};
+        }
+        u = ue;
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_attn_tile_join(AttnArgs a, int n_wg) {
+    __shared__ Axis axis;
+    const int g = (int)blockIdx.x + 1, hd = a.hd, G = a.group.d;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+    axis_init<true>(a, axis);
+    const Split split(axis.total, n_wg);
+    const long u = split.first(g);
+    if (u >= axis.total || u == 0) return;
+    const Item it = axis_item<true>(a, axis, u);
+    if (it.a >= u || split.first(g - 1) > it.a) return;
+    int last = g;
+    while (split.first(last + 1) < it.b) last++;
+    const int tt = a.tile_tokens, t0 = it.tile * tt;
+    const int mrow = wave * 32 + col, tok = t0 + a.group.quot(mrow), row = it.r.row0 + tok;
+    if (!(mrow < tt * G && tok < it.r.n && (unsigned)row < (unsigned)a.rows)) return;
+    const long head = it.kvh * G + mrow - (tok - t0) * G;
+    float m = -INFINITY, l = 0.0f;
+    f4v o[4 * DT];
+#pragma unroll
+    for (int i = 0; i < 4 * DT; i++) o[i] = f4v{0.f, 0.f, 0.f, 0.f};
+    for (int w = g - 1; w <= last; w++) {
+        const float *part = a.parts + (long)(2 * w + (w == g - 1)) * tile_part(DT);
+        const f4v *po = reinterpret_cast<const f4v *>(part) + (long)wave * 4 * DT * 64 + lane;
+        const f2v ml = *reinterpret_cast<const f2v *>(part + kTileRows * 32 * DT + 2 * mrow);
+        const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
+        const float f = exp2_hw(m - ref), pf = exp2_hw(ml.x - ref);
+        l = l * f + ml.y * pf;
         m = mn;
-        ps[lane] = p;
-        at[lane] = off;
-        __syncthreads();
-        o[0] *= f; o[1] *= f;
-        for (int j = 0; j < 64; j++) {
-            if (at[j] < 0) continue;
-            for (int t = 0; t < 2; t++) {
-                const int d = lane + 64 * t;
-                if (d >= a.hd) continue;
-                const float4 x = get4<BF16>(a.v, at[j] + (d & ~3));
-                const float v = d & 2 ? (d & 1 ? x.w : x.z) : (d & 1 ? x.y : x.x);
-                o[t] = fmaf(ps[j], v, o[t]);
-            }
-        }
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4 * DT; i++) o[i] = o[i] * f + po[i * 64] * pf;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    for (int t = 0; t < 2; t++)
-        if (lane + 64 * t < a.hd) a.out[r * a.ldo + (long)h * a.hd + lane + 64 * t] = o[t] * inv;
+    float *out = a.out + row * a.ldo + head * hd;
+#pragma unroll
+    for (int i = 0; i < 4 * DT; i++) {
+        const int at = 32 * (i >> 2) + 8 * (i & 3) + 4 * half;
+        if (at < hd) *reinterpret_cast<f4v *>(out + at) = o[i] * inv;
+    }
+}
+
+// ── launch ───────────────────────────────────────────────────────────────
+constexpr int kFewGroups = 1024, kTileGroups = 512;         // workgroups: what the chip holds at once
+
+int few_hq(int hd) { return hd <= 32 ? 2 : hd <= 64 ? 4 : hd <= 96 ? 6 : 8; }
+int tile_dt(int hd) { return (hd + 31) / 32; }
+
+typedef void (*Fn)(AttnArgs);
+typedef void (*JoinFn)(AttnArgs, int);
+
+template <int HQ>
+Fn few_fn(int hd, bool b16) {
+    return hd == 16 * HQ ? (b16 ? k_attn_few<HQ, false, true> : k_attn_few<HQ, false, false>)
+                         : (b16 ? k_attn_few<HQ, true, true> : k_attn_few<HQ, true, false>);
+}
+
+bool may_have_tiles(int group, int max_new) { return max_new == 0 || (long)max_new * group > kFewRows; }
+
+size_t work_floats(const ptmi_pages_t &p, int n_heads, int max_new, size_t *tile_at) {
+    size_t n = (size_t)2 * kFewGroups * few_part(few_hq(p.head_dim));
+    *tile_at = n;
+    if (may_have_tiles(n_heads / p.n_kv_heads, max_new)) n += (size_t)2 * kTileGroups * tile_part(tile_dt(p.head_dim));
+    return n;
 }
 
 int check_heads(const char *who, const ptmi_pages_t *pages, int n_heads, int max_new) {
     int st = check_pages(who, pages);
     if (st) return st;
-    if (n_heads < 1 || n_heads % pages->n_kv_heads || n_heads > 65535)
+    if (n_heads < 1 || n_heads % pages->n_kv_heads || n_heads / pages->n_kv_heads > kTileRows)
         return set_error(PTMI_ERR_ARG, "%s: n_heads=%d for n_kv_heads=%d", who, n_heads, pages->n_kv_heads);
     if (max_new < 0) return set_error(PTMI_ERR_ARG, "%s: max_new=%d", who, max_new);
     return PTMI_OK;
@@ -117,7 +933,8 @@ extern "C" {
 
 size_t ptmi_paged_attention_work(const ptmi_pages_t *pages, int n_heads, int max_new) {
     if (check_heads("ptmi_paged_attention_work", pages, n_heads, max_new)) return 0;
-    return 16;
+    size_t tile_at;
+    return work_floats(*pages, n_heads, max_new, &tile_at) * sizeof(float);
 }
 
 int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, int table_width,
@@ -130,6 +947,8 @@ int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, 
     if (n_requests < 0 || table_width < 1 || rows < 0 || !std::isfinite(scale))
         return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: n_requests=%d table_width=%d rows=%d scale=%g", n_requests,
                          table_width, rows, (double)scale);
+    if ((long long)table_width * p.page_size > INT_MAX - 4096)
+        return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: %d pages of %d positions a request", table_width, p.page_size);
     if (n_requests == 0 || rows == 0) return PTMI_OK;
     if (!block_table || !row_start || !kv_len || !q || !out || !work)
         return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: NULL argument");
@@ -138,19 +957,40 @@ int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, 
         return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: rows must be 16-byte aligned and hold %d heads (ldq=%ld ldo=%ld)",
                          n_heads, ldq, ldo);
     if (q == out) return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: out must not be q");
-    const size_t need = ptmi_paged_attention_work(pages, n_heads, max_new);
+    size_t tile_at;
+    const size_t need = work_floats(p, n_heads, max_new, &tile_at) * sizeof(float);
     if (work_bytes < need)
         return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: work holds %zu bytes, %zu needed", work_bytes, need);
     if ((st = ensure_init())) return st;
     DeviceScope dev;
     if ((st = dev.enter())) return st;
-    const AttnArgs a = {p.k, p.v, p.page_stride, p.pos_stride, p.head_stride, p.n_pages, FastDiv(p.page_size),
-                        block_table, table_width, row_start, kv_len, n_requests, q, ldq, out, ldo, rows, n_heads,
-                        p.n_kv_heads, p.head_dim, scale};
+    const int group = n_heads / p.n_kv_heads;
+    AttnArgs a = {p.k, p.v, p.page_stride, p.pos_stride, p.head_stride, p.n_pages, FastDiv(p.page_size), block_table,
+                  table_width, row_start, kv_len, n_requests, q, ldq, out, ldo, rows, p.n_kv_heads, p.head_dim,
+                  FastDiv(group), kTileRows / group, scale * 1.44269504088896341f, (float *)work};
     hipStream_t s = stream ? (hipStream_t)stream : lib_stream();
-    hipLaunchKernelGGL(p.type == PTMI_BF16 ? k_attn_simple<true> : k_attn_simple<false>, dim3(rows, n_heads), dim3(64),
-                       0, s, a);
-    PTMI_HIP(hipGetLastError());
+    const bool b16 = p.type == PTMI_BF16;
+    if (group <= kFewRows) {
+        const int hq = few_hq(p.head_dim);
+        const Fn fn = hq == 2 ? few_fn<2>(p.head_dim, b16) : hq == 4 ? few_fn<4>(p.head_dim, b16)
+                    : hq == 6 ? few_fn<6>(p.head_dim, b16) : few_fn<8>(p.head_dim, b16);
+        hipLaunchKernelGGL(fn, dim3(kFewGroups), dim3(kThreads), 0, s, a);
+        // no head has more than one unit: nothing to join
+        if ((long)table_width * p.page_size > kUnit)
+            hipLaunchKernelGGL(hq <= 4 ? k_attn_few_join<4> : k_attn_few_join<8>, dim3(kFewGroups - 1), dim3(kThreads), 0,
+                               s, a, kFewGroups);
+        PTMI_HIP(hipGetLastError());
+    }
+    if (may_have_tiles(group, max_new)) {
+        a.parts = (float *)work + tile_at;
+        static const Fn fns[4][2] = {{k_attn_tile<1, false>, k_attn_tile<1, true>}, {k_attn_tile<2, false>, k_attn_tile<2, true>},
+                                     {k_attn_tile<3, false>, k_attn_tile<3, true>}, {k_attn_tile<4, false>, k_attn_tile<4, true>}};
+        static const JoinFn joins[4] = {k_attn_tile_join<1>, k_attn_tile_join<2>, k_attn_tile_join<3>, k_attn_tile_join<4>};
+        const int dt = tile_dt(p.head_dim);
+        hipLaunchKernelGGL(fns[dt - 1][b16], dim3(kTileGroups), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL(joins[dt - 1], dim3(kTileGroups - 1), dim3(kThreads), 0, s, a, kTileGroups);
+        PTMI_HIP(hipGetLastError());
+    }
     return PTMI_OK;
 }
 

@@ -67,7 +67,8 @@ def test_store_refuses(bad):
 @pytest.mark.parametrize("bad", [dict(n=-1), dict(width=0), dict(rows=-1), dict(new=-1), dict(heads=0), dict(heads=3),
                                  dict(scale=float("nan")), dict(scale=float("inf")), dict(table=None), dict(start=None),
                                  dict(kv=None), dict(q=None), dict(out=None), dict(work=None), dict(q=P + 4), dict(out=P),
-                                 dict(ldq=252), dict(ldo=257), dict(work=P + 8), dict(work_bytes=0)], ids=str)
+                                 dict(ldq=252), dict(ldo=257), dict(work=P + 8), dict(work_bytes=0),
+                                 dict(width=1 << 27)], ids=str)
 def test_attention_refuses(bad):
     assert attend(cache(), **bad) == ARG
 
