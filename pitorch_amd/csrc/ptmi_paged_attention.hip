@@ -33,7 +33,7 @@ typedef float f2v __attribute__((ext_vector_type(2)));
 
 constexpr int kUnit = 64;            // keys of a unit
 constexpr int kFewRows = 16;         // rows of k_attn_few
-constexpr int kTileRows = 128;       // rows of a tile of k_attn_tile
+constexpr int kTileRows = 128;       // least rows of a tile of k_attn_tile
 constexpr int kThreads = 256;
 
 struct AttnArgs {
@@ -47,8 +47,9 @@ struct AttnArgs {
     float *out; long ldo;
     int rows, kv_heads, hd;
     FastDiv group;                   // query heads of a key head
-    int tile_tokens;                 // tokens of a tile: whole tokens of at most kTileRows rows
+    int tile_tokens;                 // tokens of a tile: those whose rows it holds whole
     float qscale;                    // scale * log2(e)
+    float minus_one;
     float *parts;                    // parts of heads cut between workgroups
 };
 
@@ -63,97 +64,107 @@ __device__ __forceinline__ Request request(const AttnArgs &a, int s) {
     return r;
 }
 
-// sum_{i<n} floor((a i + b) / 64)
-__device__ long floor_sum(unsigned n, unsigned a, unsigned b) {
-    long sum = 0;
-    unsigned m = kUnit;
-    for (;;) {
-        sum += (long)n * (n - 1) / 2 * (a / m) + (long)n * (b / m);
-        a %= m;
-        b %= m;
-        const unsigned long y = (unsigned long)a * n + b;
-        if (y < m) return sum;
-        n = (unsigned)(y / m);
-        b = (unsigned)(y % m);
-        const unsigned t = m;
-        m = a;
-        a = t;
-    }
+__device__ __forceinline__ long quotient(long a, long b) { // 32 bits where they do
+    return (a | b) < UINT_MAX ? (long)((unsigned)a / (unsigned)b) : a / b;
 }
 
-// Units of one key head of a request; 0: the other kernel's.  A tile of
-// rows counts the keys its last whole token would see: at most a unit or
-// two too many at the request's end, which find no key and cost nothing.
+// Units of one key head of a request; 0: the other kernel's.  Tile i of rows
+// has floor((b + i tt)/64) of them, tt its tokens: the keys its last whole
+// token would see, at most a unit or two too many at the request's end, which
+// find no key and cost nothing.  64 tiles on, a tile has tt units more.
 __device__ __forceinline__ unsigned tile_keys0(const AttnArgs &a, const Request &r) {
     return (unsigned)max(r.len - r.n, 0) + a.tile_tokens + kUnit - 1;
 }
+// Units of the 64 k tiles before block k of 64, if block 0 has s.
+__device__ __forceinline__ long blocks_before(long k, long s, int tt) { return k * s + 32 * tt * k * (k - 1); }
+
 template <bool TILE>
 __device__ __forceinline__ long head_units(const AttnArgs &a, const Request &r) {
     const bool few = (long)r.n * a.group.d <= kFewRows;
     if (r.n == 0 || few == TILE) return 0;
-    if constexpr (TILE)
-        return floor_sum((r.n + a.tile_tokens - 1) / a.tile_tokens, a.tile_tokens, tile_keys0(a, r));
-    else
+    if constexpr (TILE) {
+        const int tt = a.tile_tokens, tiles = (r.n + tt - 1) / tt, k = tiles >> 6, rest = tiles & 63;
+        const unsigned b0 = tile_keys0(a, r);
+        long s = 0, s_rest = 0;
+        for (int i = 0; i < (k ? 64 : rest); i++) {
+            s += (b0 + (unsigned)(i * tt)) / kUnit;
+            if (i + 1 == rest) s_rest = s;
+        }
+        return blocks_before(k, s, tt) + s_rest + (long)rest * tt * k;
+    } else {
         return max(1, (r.len + kUnit - 1) / kUnit);
+    }
 }
 
-// The units of 256 requests at a time, as sums in shared memory.
+// The units of 256 requests at a time, as sums in shared memory, and the requests.
 struct Axis {
     long pre[kThreads + 1];          // units before request c0 + i
-    long total;                      // of all requests
+    Request req[kThreads];
+    long wsum[kThreads / 64];
     int c0;
 };
 
-__device__ __forceinline__ long wave_scan(long v) {        // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
+// Inclusive sums over the wave by DPP: within rows of 16 lanes, then each
+// row's (half's) last lane to the next row (half).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ long dpp_add(long v) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
+    return v + (long)((unsigned long)hi << 32 | lo);
+}
+__device__ __forceinline__ long wave_scan(long v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    return dpp_add<0x143, 0xC>(v);
 }
 
-// Fills x for requests [c0, c0 + 256) after `before` units; every thread takes part.
+// Fills x for requests [c0, c0 + 256) after `before` units; all threads of
+// the block take part, the first 256 hold a request each.
 template <bool TILE>
 __device__ void axis_fill(const AttnArgs &a, Axis &x, int c0, long before) {
-    __shared__ long wsum[kThreads / 64];
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+    const bool mine = t < kThreads;
     long v = 0;
-    if (c0 + t < a.n_req) v = head_units<TILE>(a, request(a, c0 + t)) * a.kv_heads;
+    Request r = {0, 0, 0};
+    if (mine && c0 + t < a.n_req) {
+        r = request(a, c0 + t);
+        v = head_units<TILE>(a, r) * a.kv_heads;
+    }
     const long incl = wave_scan(v);
     __syncthreads();
-    if (lane == 63) wsum[w] = incl;
+    if (mine) {
+        x.req[t] = r;
+        if (lane == 63) x.wsum[w] = incl;
+    }
     __syncthreads();
-    for (int i = 0; i < w; i++) before += wsum[i];
-    x.pre[t + 1] = before + incl;
-    if (t == 0) { x.pre[0] = before; x.c0 = c0; }
+    if (mine) {
+        for (int i = 0; i < w; i++) before += x.wsum[i];
+        x.pre[t + 1] = before + incl;
+        if (t == 0) { x.pre[0] = before; x.c0 = c0; }
+    }
     __syncthreads();
 }
 
 // Counts all units; x then holds the requests' first 256.
 template <bool TILE>
-__device__ void axis_init(const AttnArgs &a, Axis &x) {
-    if (a.n_req > kThreads) {
-        long total = 0;
+__device__ long axis_init(const AttnArgs &a, Axis &x) {
+    long total = 0;
+    if (a.n_req > kThreads)
         for (int c0 = 0; c0 < a.n_req; c0 += kThreads) {
             axis_fill<TILE>(a, x, c0, total);
             total = x.pre[kThreads];
         }
-        axis_fill<TILE>(a, x, 0, 0);
-        if (threadIdx.x == 0) x.total = total;
-    } else {
-        axis_fill<TILE>(a, x, 0, 0);
-        if (threadIdx.x == 0) x.total = x.pre[kThreads];
-    }
-    __syncthreads();
+    axis_fill<TILE>(a, x, 0, 0);
+    return a.n_req > kThreads ? total : x.pre[kThreads];
 }
 
 // The request that holds unit u < total (refills x as needed).
 template <bool TILE>
 __device__ int axis_find(const AttnArgs &a, Axis &x, long u) {
     while (u >= x.pre[kThreads]) axis_fill<TILE>(a, x, x.c0 + kThreads, x.pre[kThreads]);
-    while (u < x.pre[0]) axis_fill<TILE>(a, x, 0, 0);       // (only ever walked forward)
     int lo = 0, hi = kThreads;                              // pre[lo] <= u < pre[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -166,10 +177,7 @@ __device__ int axis_find(const AttnArgs &a, Axis &x, long u) {
 // The stretches: workgroup g of n takes units [first(g), first(g + 1)).
 struct Split {
     long each, more;                 // the first `more` take each + 1
-    __device__ Split(long total, int n) {
-        each = total < INT_MAX ? (long)((unsigned)total / (unsigned)n) : total / n;
-        more = total - each * n;
-    }
+    __device__ Split(long total, int n) : each(quotient(total, n)), more(total - each * n) {}
     __device__ long first(int g) const { return g * each + min((long)g, more); }
 };
 
@@ -183,23 +191,24 @@ template <bool TILE>
 __device__ Item axis_item(const AttnArgs &a, Axis &x, long u) {
     Item it;
     it.s = axis_find<TILE>(a, x, u);
-    it.r = request(a, it.s);
+    it.r = x.req[it.s - x.c0];
     const long per = head_units<TILE>(a, it.r), base = x.pre[it.s - x.c0];
-    it.kvh = (int)((u - base) / per);
+    it.kvh = (int)quotient(u - base, per);
     it.a = base + it.kvh * per;
     it.b = it.a + per;
     it.tile = 0;
-    if constexpr (TILE) {
-        const unsigned tt = a.tile_tokens, b0 = tile_keys0(a, it.r);
-        unsigned lo = 0, hi = (it.r.n + tt - 1) / tt;       // sum(lo) <= u - a < sum(hi)
-        while (hi - lo > 1) {
-            const unsigned mid = (lo + hi) >> 1;
-            if (floor_sum(mid, tt, b0) <= u - it.a) lo = mid;
-            else hi = mid;
-        }
-        it.tile = (int)lo;
-        it.a += floor_sum(lo, tt, b0);
-        it.b = it.a + (long)((b0 + lo * tt) / kUnit);
+    if constexpr (TILE) {                                  // lane i: tile 64 k + i
+        const int tt = a.tile_tokens, lane = threadIdx.x & 63;
+        const long mine = (tile_keys0(a, it.r) + (unsigned)(lane * tt)) / kUnit, upto = wave_scan(mine);
+        const long s = __shfl(upto, 63);
+        long k = 0, w = u - it.a;
+        while (blocks_before(k + 1, s, tt) <= w) k++;
+        w -= blocks_before(k, s, tt);
+        const long end = upto + (long)(lane + 1) * tt * k;
+        const int i = __popcll(__ballot(end <= w));         // (under 64: w lies in block k)
+        it.tile = (int)(64 * k) + i;
+        it.b = it.a + blocks_before(k, s, tt) + __shfl(end, i);
+        it.a = it.b - __shfl(mine, i) - tt * k;
     }
     return it;
 }
@@ -244,8 +253,21 @@ __device__ __forceinline__ int page_of(const AttnArgs &a, int s, int key, int li
     return key < limit ? a.table[(long)s * a.width + a.page.quot(key)] : -1;
 }
 
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ bool finite_bits(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+// Values that are not finite as 0.
+__device__ __forceinline__ void drop_odd(Raw4<false> &r) {
+    r.x = make_float4(finite_bits(r.x.x) ? r.x.x : 0.f, finite_bits(r.x.y) ? r.x.y : 0.f,
+                      finite_bits(r.x.z) ? r.x.z : 0.f, finite_bits(r.x.w) ? r.x.w : 0.f);
+}
+__device__ __forceinline__ void drop_odd(Raw4<true> &r) {
+    const f4v x = widen(r);
+    if (!finite_bits(x.x)) r.x.x &= 0xFFFF0000u;
+    if (!finite_bits(x.y)) r.x.x &= 0x0000FFFFu;
+    if (!finite_bits(x.z)) r.x.y &= 0xFFFF0000u;
+    if (!finite_bits(x.w)) r.x.y &= 0x0000FFFFu;
+}
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ── few rows ─────────────────────────────────────────────────────────────
 // v_mfma_f32_16x16x4_f32: lane l supplies A[l%16][l/16] and B[l/16][l%16];
@@ -260,9 +282,9 @@ __device__ __forceinline__ f4v mfma4(float a, float b, f4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Floats of a part: o [16][pitch], then (m, l) [16].
-constexpr int few_pitch(int hq) { return hq > 4 ? 128 : 64; }
-constexpr int few_part(int hq) { return kFewRows * few_pitch(hq) + 2 * kFewRows; }
+// Floats of a part: o [16][pitch], then (m, l) [16] (dt = head_dim / 32, rounded up).
+constexpr int few_pitch(int dt) { return dt > 2 ? 128 : 64; }
+constexpr int few_part(int dt) { return kFewRows * few_pitch(dt) + 2 * kFewRows; }
 
 template <int HQ, bool PAD, bool BF16>
 struct FewBlock {                    // 16 keys of one head
@@ -294,14 +316,13 @@ __device__ __forceinline__ void few_load(const AttnArgs &a, FewBlock<HQ, PAD, BF
 
 template <int HQ, bool PAD, bool BF16>
 __global__ __launch_bounds__(kThreads) void k_attn_few(AttnArgs a) {
-    constexpr int C4 = HQ > 4 ? 2 : 1, NC = 4 * C4, PITCH = few_pitch(HQ) + 4, NW = kThreads / 64;
+    constexpr int C4 = HQ > 4 ? 2 : 1, NC = 4 * C4, FP = few_pitch(HQ / 2), PITCH = FP + 4, NW = kThreads / 64;
     __shared__ Axis axis;
     __shared__ __align__(16) float red[NW * kFewRows * PITCH];
     __shared__ float st_m[NW][kFewRows], st_l[NW][kFewRows];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
     const int hd = PAD ? a.hd : 16 * HQ, n4 = hd >> 2, G = a.group.d;
-    axis_init<false>(a, axis);
-    const Split split(axis.total, gridDim.x);
+    const Split split(axis_init<false>(a, axis), gridDim.x);
     const int wg = stretch_of_block();
     const long u1 = split.first(wg + 1);
     for (long u = split.first(wg); u < u1;) {
@@ -423,7 +444,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_few(AttnArgs a) {
         }
         __syncthreads();
         const bool whole = u == it.a && ue == it.b;
-        float *part = a.parts + (long)(2 * wg + (u == it.a)) * few_part(HQ);
+        float *part = a.parts + (long)(2 * wg + (u == it.a)) * few_part(HQ / 2);
         for (int e = threadIdx.x; e < M * n4; e += kThreads) {
             const int i = e / n4, c = e - i * n4;
             f4v o = *reinterpret_cast<const f4v *>(red + i * PITCH + 4 * c);
@@ -441,52 +462,15 @@ __global__ __launch_bounds__(kThreads) void k_attn_few(AttnArgs a) {
                     *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(it.kvh * G + i - t * G) * hd + 4 * c) =
                         o * (il == 0.0f ? 0.0f : 1.0f / il);
             } else {
-                *reinterpret_cast<f4v *>(part + i * few_pitch(HQ) + 4 * c) = o;
+                *reinterpret_cast<f4v *>(part + i * FP + 4 * c) = o;
                 if (c == 0) {
-                    part[kFewRows * few_pitch(HQ) + 2 * i] = im;
-                    part[kFewRows * few_pitch(HQ) + 2 * i + 1] = il;
+                    part[kFewRows * FP + 2 * i] = im;
+                    part[kFewRows * FP + 2 * i + 1] = il;
                 }
             }
         }
         __syncthreads();
         u = ue;
-    }
-}
-
-// Joins the parts of heads that workgroup boundaries cut: block g takes the
-// head that boundary g cuts, if no earlier boundary does.
-template <int HQ>
-__global__ __launch_bounds__(kThreads) void k_attn_few_join(AttnArgs a, int n_wg) {
-    __shared__ Axis axis;
-    const int g = (int)blockIdx.x + 1, hd = a.hd, n4 = hd >> 2, G = a.group.d;
-    axis_init<false>(a, axis);
-    const Split split(axis.total, n_wg);
-    const long u = split.first(g);
-    if (u >= axis.total || u == 0) return;
-    const Item it = axis_item<false>(a, axis, u);
-    if (it.a >= u || split.first(g - 1) > it.a) return;
-    const int M = it.r.n * G;
-    int last = g;                                           // the workgroup of the head's last unit
-    while (split.first(last + 1) < it.b) last++;
-    auto part_of = [&](int w) { return a.parts + (long)(2 * w + (w == g - 1)) * few_part(HQ); };
-    for (int e = threadIdx.x + blockIdx.y * kThreads; e < M * n4; e += kThreads * gridDim.y) {
-        const int i = e / n4, c = e - i * n4;
-        float m = -INFINITY, l = 0.0f;
-        f4v o = {0.f, 0.f, 0.f, 0.f};
-        for (int w = g - 1; w <= last; w++) {
-            const float *p = part_of(w);
-            const float pm = p[kFewRows * few_pitch(HQ) + 2 * i], pl = p[kFewRows * few_pitch(HQ) + 2 * i + 1];
-            const f4v po = *reinterpret_cast<const f4v *>(p + i * few_pitch(HQ) + 4 * c);
-            const float mn = fmaxf(m, pm), ref = mn == -INFINITY ? 0.0f : mn;
-            const float f = exp2_hw(m - ref), pf = exp2_hw(pm - ref);
-            l = l * f + pl * pf;
-            o = o * f + po * pf;
-            m = mn;
-        }
-        const int t = a.group.quot(i), r = it.r.row0 + t;
-        if ((unsigned)r < (unsigned)a.rows)
-            *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(it.kvh * G + i - t * G) * hd + 4 * c) =
-                o * (l == 0.0f ? 0.0f : 1.0f / l);
     }
 }
 
@@ -509,7 +493,6 @@ constexpr int kTop = 14;             // largest |h| < 2^15
 constexpr int kBias = 9;             // weights are held times 2^9:
 constexpr float kLazy = 6.0f;        // a maximum up to 2^6 above m does not move m (2^15 < 65504)
 
-constexpr int tile_part(int dt) { return kTileRows * (32 * dt + 2); }    // floats
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(min(max(e, -126), 127) + 127) << 23); }
 
@@ -520,31 +503,95 @@ __device__ __forceinline__ h2v cvt2(float x, float y) {
     const f2v v = {x, y};
     return __builtin_convertvector(v, h2v);
 }
-__device__ __forceinline__ h2v rest2(float x, float y, h2v h) {
-    return cvt2(fmaf((float)h.x, -1.0f, x), fmaf((float)h.y, -1.0f, y));
+// (x, y) s as h + l.  minus_one: -1, of a value the compiler does not know, so
+// that each l is one fused operation on both precisions (a subtraction would
+// be two and a packing).
+__device__ __forceinline__ void split2(float x, float y, float minus_one, h2v &h, h2v &l) {
+    h = cvt2(x, y);
+    l = h2v{(_Float16)fmaf((float)h.x, minus_one, x), (_Float16)fmaf((float)h.y, minus_one, y)};
 }
+__device__ __forceinline__ void split4(const f4v &x, float minus_one, h4v &h, h4v &l) {
+    h2v h0, h1, l0, l1;
+    split2(x.x, x.y, minus_one, h0, l0);
+    split2(x.z, x.w, minus_one, h1, l1);
+    h = h4v{h0.x, h0.y, h1.x, h1.y};
+    l = h4v{l0.x, l0.y, l1.x, l1.y};
+}
+// The largest magnitude seen, of any bits: the largest bits as unsigned (of
+// the negative ones, if any) and as signed (of the positive ones, if any).
+struct TopBits {
+    unsigned u = 0;
+    int i = 0;
+    __device__ __forceinline__ void add(const f4v &x) {
+        u = max(max(u, __float_as_uint(x.x)), max(max(__float_as_uint(x.y), __float_as_uint(x.z)), __float_as_uint(x.w)));
+        i = max(max(i, __float_as_int(x.x)), max(max(__float_as_int(x.y), __float_as_int(x.z)), __float_as_int(x.w)));
+    }
+    __device__ __forceinline__ unsigned bits() const { return max(u & 0x7FFFFFFFu, (unsigned)i & 0x7FFFFFFFu); }
+};
+// The upper halves of two magnitudes' bits, and the wave's largest of each
+// (enough for the exponent, and to tell infinities and NaN).
+typedef unsigned short u2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u2v top_halves(unsigned k, unsigned v) {
+    return __builtin_bit_cast(u2v, (k >> 16) | (v & 0xFFFF0000u));
+}
+template <int CTRL>
+__device__ __forceinline__ u2v dpp_max(u2v x) {
+    const unsigned o = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true);
+    return __builtin_elementwise_max(x, __builtin_bit_cast(u2v, o));
+}
+__device__ __forceinline__ u2v wave_top(u2v x) {
+    x = dpp_max<0xB1>(x);
+    x = dpp_max<0x4E>(x);
+    x = dpp_max<0x141>(x);
+    x = dpp_max<0x140>(x);
+    int hi, lo = pl16i(__builtin_bit_cast(int, x), hi);
+    x = __builtin_elementwise_max(__builtin_bit_cast(u2v, lo), __builtin_bit_cast(u2v, hi));
+    lo = pl32i(__builtin_bit_cast(int, x), hi);
+    return __builtin_elementwise_max(__builtin_bit_cast(u2v, lo), __builtin_bit_cast(u2v, hi));
+}
+constexpr unsigned kNotFinite = 0x7F80;                     // upper half of an infinity's bits
+__device__ __forceinline__ unsigned finite_top(unsigned top, const f4v &x) {
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (finite_bits(x[e])) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+    return top;
+}
+
+constexpr int tile_waves(int dt) { return dt <= 2 ? 4 : 8; }
+constexpr int tile_part(int dt) { return 32 * tile_waves(dt) * (32 * dt + 2); }   // floats
 
 template <int DT, bool BF16>
 struct TileLds {
     static constexpr int HP = 32 * DT, KP = HP + 8, VP = kUnit + 8;      // pitches in halves
     static constexpr int PL = BF16 ? 1 : 2;                              // planes: h, l
-    _Float16 k[PL][kUnit * KP], v[PL][HP * VP];
-    long off[4][kUnit];              // units u..u+3: offsets of their keys, -1: not there
+    _Float16 k[2][PL][kUnit * KP], v[2][PL][HP * VP];                    // units b and b + 1
+    long off[4][kUnit];              // units b..b+3: offsets of their keys, -1: not there
     int all[4];                      // whether all 64 are
-    unsigned kmax[2][4], vmax[2][4];
+    unsigned top[2][tile_waves(DT)]; // each wave's top_halves of the unit in flight
+    int odd[4];                      // whether one of their values is not finite
 };
 
-template <int DT, bool BF16>
-__global__ __launch_bounds__(kThreads, DT <= 2 ? 2 : 1) void k_attn_tile(AttnArgs a) {
+// Where in its 64 keys a value row keeps quad `place`: rows 16 apart, whose
+// writes would meet in one bank, use different 16-key groups.
+__device__ __forceinline__ int vplace(int row, int place) { return place ^ ((row >> 4 & 3) << 2); }
+
+// NW waves of 32 rows; PAD: head_dim is not 32 DT (slots past it are zero).
+// While unit b's products run, unit b + 1 is split into shared memory (its
+// other half) and unit b + 2 is on its way to registers: one barrier a unit.
+template <int DT, bool PAD, bool BF16>
+__global__ __launch_bounds__(64 * tile_waves(DT), 2) void k_attn_tile(AttnArgs a) {
     typedef TileLds<DT, BF16> Lds;
-    constexpr int HP = Lds::HP, KP = Lds::KP, VP = Lds::VP, PL = Lds::PL, KS = HP / 16;
-    constexpr int VT = (128 * DT + kThreads - 1) / kThreads;             // value tasks of a thread: 4 keys x 4 columns
+    constexpr int HP = Lds::HP, KP = Lds::KP, VP = Lds::VP, PL = Lds::PL, KS = HP / 16, NW = tile_waves(DT), NT = 64 * NW;
+    constexpr int C = 8 * DT;                                            // float4s of a row
+    constexpr int KL = NT / kUnit, KT = (C + KL - 1) / KL;               // threads of a key row, float4s of each
+    constexpr int VT = (16 * C + NT - 1) / NT;                           // value tasks of a thread: 4 keys x 4 columns
+    static_assert(C % KL == 0, "every key thread has the same float4s");
     __shared__ Axis axis;
     __shared__ __align__(16) Lds lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-    const int hd = a.hd, n4 = hd >> 2, G = a.group.d;
-    axis_init<true>(a, axis);
-    const Split split(axis.total, gridDim.x);
+    const int hd = PAD ? a.hd : HP, n4 = hd >> 2, G = a.group.d;
+    const float m1 = a.minus_one;
+    const Split split(axis_init<true>(a, axis), gridDim.x);
     const int wg = stretch_of_block();
     const long u1 = split.first(wg + 1);
     for (long u = split.first(wg); u < u1;) {
@@ -555,50 +602,13 @@ __global__ __launch_bounds__(kThreads, DT <= 2 ? 2 : 1) void k_attn_tile(AttnArg
         // this lane's row of the tile
         const int mrow = wave * 32 + col, tok = t0 + a.group.quot(mrow), row = it.r.row0 + tok;
         const bool live = mrow < tt * G && tok < it.r.n && (unsigned)row < (unsigned)a.rows;
+        const bool busy = __any(live);                       // this wave has rows
         const long head = it.kvh * G + mrow - (tok - t0) * G;
         const int see = it.r.len - it.r.n + tok + 1;        // its keys: [0, see)
         const int see0 = it.r.len - it.r.n + t0 + 1;        // of the tile's first row
-        // q: columns 16 ks + 8 half .. of the row, scaled, split
-        h8v qh[KS], ql[KS];
-        int qe;
-        {
-            float x[KS][8];
-            float top = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    f4v v = {0.f, 0.f, 0.f, 0.f};
-                    const int d = 16 * ks + 8 * half + 4 * j;
-                    if (live && d < hd) v = *reinterpret_cast<const f4v *>(a.q + row * a.ldq + head * hd + d) * a.qscale;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[ks][4 * j + e] = v[e];
-                        top = finite_bits(v[e]) ? fmaxf(top, fabsf(v[e])) : top;
-                    }
-                }
-            const LanePair pr = pl32(top);
-            qe = max((int)(__float_as_uint(fmaxf(pr.lo, pr.hi)) >> 23) - 127, -100) - kTop;
-            const float sc = pow2(-qe);
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float y0 = x[ks][2 * j] * sc, y1 = x[ks][2 * j + 1] * sc;
-                    const h2v h = cvt2(y0, y1), r = rest2(y0, y1, h);
-                    qh[ks][2 * j] = h.x; qh[ks][2 * j + 1] = h.y;
-                    ql[ks][2 * j] = r.x; ql[ks][2 * j + 1] = r.y;
-                }
-        }
-        f16v acc[DT];
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) acc[d][r] = 0.0f;
-        float m = -INFINITY, l = 0.0f;
-        int ve = -1000;                                      // acc holds values times 2^-ve
         const int b0 = (int)(u - it.a), b1 = (int)min((long)(end + kUnit - 1) / kUnit, ue - it.a);   // units of keys
-        // Offsets of unit b's keys go to slot b & 3 two units ahead of their use, page numbers one further.
+        // Offsets of unit b's keys go to slot b & 3 a barrier ahead of their use.  Wave b % NW does unit b, with
+        // page numbers that it asked for NW units before.
         auto put_off = [&](int b, int pg) {
             const long off = b < b1 ? key_offset(a, b * kUnit + lane, end, pg, it.kvh) : -1;
             lds.off[b & 3][lane] = off;
@@ -606,220 +616,282 @@ __global__ __launch_bounds__(kThreads, DT <= 2 ? 2 : 1) void k_attn_tile(AttnArg
             if (lane == 0) lds.all[b & 3] = all;
         };
         auto page_at = [&](int b) { return b < b1 ? page_of(a, it.s, b * kUnit + lane, end) : -1; };
-        int pg = -1;
+        const int turn = (wave - b0) & (NW - 1);             // this wave's first unit, from b0
+        int pg = page_at(b0 + turn);
         __syncthreads();                                     // the last item's readers are done
-        if (wave == 0) {
-            const int p0 = page_at(b0), p1 = page_at(b0 + 1);
-            pg = page_at(b0 + 2);
-            put_off(b0, p0);
-            put_off(b0 + 1, p1);
+        if (turn < 3) {
+            put_off(b0 + turn, pg);
+            pg = page_at(b0 + turn + NW);
         }
-        __syncthreads();
-        Raw4<BF16> rk[HP / 16], rv[VT][4];
-        auto load = [&](int b) {
-            const long *off = lds.off[b & 3];
-            const long ko = off[tid >> 2];
-#pragma unroll
-            for (int j = 0; j < HP / 16; j++) {
-                const int i = (tid & 3) + 4 * j;
-                rk[j] = raw_zero<BF16>();
-                if (ko >= 0 && i < n4) rk[j] = raw_load<BF16>(a.k, ko + 4 * i);
-            }
-#pragma unroll
-            for (int t = 0; t < VT; t++) {
-                const int task = tid + t * kThreads, quad = task / (8 * DT), c = task % (8 * DT);
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    rv[t][s] = raw_zero<BF16>();
-                    if (quad < 16 && c < n4) {
-                        const long vo = off[4 * quad + s];
-                        if (vo >= 0) rv[t][s] = raw_load<BF16>(a.v, vo + 4 * c);
-                    }
-                }
-            }
-        };
-        if (b0 < b1) load(b0);
-        for (int b = b0; b < b1; b++) {
-            // the largest exponents of the unit
-            unsigned km = 0, vm = 0;
-#pragma unroll
-            for (int j = 0; j < HP / 16; j++) {
-                const f4v x = widen(rk[j]);
-#pragma unroll
-                for (int e = 0; e < 4; e++) km = max(km, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-            }
-#pragma unroll
-            for (int t = 0; t < VT; t++)
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    const f4v x = widen(rv[t][s]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) vm = max(vm, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-                }
-            float kf = group_max<64>(__uint_as_float(km >> 1)), vf = group_max<64>(__uint_as_float(vm >> 1));
-            km = __float_as_uint(kf) << 1;                   // (halved: as floats they are finite and in order)
-            vm = __float_as_uint(vf) << 1;
-            bool odd = false;                                // some value is not finite
-            if (km >= 0x7F800000u || vm >= 0x7F800000u) {    // rare: the largest finite one
-                odd = vm >= 0x7F800000u;
-                km = vm = 0;
-                for (int j = 0; j < HP / 16; j++) {
-                    const f4v x = widen(rk[j]);
-                    for (int e = 0; e < 4; e++) if (finite_bits(x[e])) km = max(km, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-                }
-                for (int t = 0; t < VT; t++)
-                    for (int s = 0; s < 4; s++) {
-                        const f4v x = widen(rv[t][s]);
-                        for (int e = 0; e < 4; e++) if (finite_bits(x[e])) vm = max(vm, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-                    }
-                km = __float_as_uint(group_max<64>(__uint_as_float(km >> 1))) << 1;
-                vm = __float_as_uint(group_max<64>(__uint_as_float(vm >> 1))) << 1;
-            }
-            if (lane == 0) {
-                lds.kmax[b & 1][wave] = km;
-                lds.vmax[b & 1][wave] = vm | (odd ? 0x80000000u : 0u);
-            }
-            __syncthreads();                                 // also: the last unit's readers are done
-            unsigned kt = 0, vt = 0, any_odd = 0;
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                kt = max(kt, lds.kmax[b & 1][w]);
-                const unsigned x = lds.vmax[b & 1][w];
-                vt = max(vt, x & 0x7FFFFFFFu);
-                any_odd |= x & 0x80000000u;
-            }
-            const int ke = max((int)(kt >> 23) - 127, -100) - kTop;
-            const int vnew = max(ve, max((int)(vt >> 23) - 127, -100) - kTop);
-            const float ks_ = pow2(-ke), vs_ = pow2(-vnew);
-#pragma unroll
-            for (int j = 0; j < HP / 16; j++) {
-                const f4v x = widen(rk[j]) * ks_;
-                const h2v h0 = cvt2(x.x, x.y), h1 = cvt2(x.z, x.w);
-                const int at = (tid >> 2) * KP + 4 * ((tid & 3) + 4 * j);
-                *reinterpret_cast<h4v *>(&lds.k[0][at]) = h4v{h0.x, h0.y, h1.x, h1.y};
-                if constexpr (PL == 2) {
-                    const h2v l0 = rest2(x.x, x.y, h0), l1 = rest2(x.z, x.w, h1);
-                    *reinterpret_cast<h4v *>(&lds.k[PL - 1][at]) = h4v{l0.x, l0.y, l1.x, l1.y};
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < VT; t++) {
-                const int task = tid + t * kThreads, quad = task / (8 * DT), c = task % (8 * DT);
-                if (quad >= 16) continue;
-                f4v x[4];
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    x[s] = widen(rv[t][s]) * vs_;
-                    if (any_odd)
-                        for (int e = 0; e < 4; e++) if (!finite_bits(x[s][e])) x[s][e] = 0.0f;
-                }
-                // quad 4 st + 2 b + h of 16 keys stands at place 4 st + 2 h + b
-                const int place = (quad & ~3) | (quad & 1) << 1 | (quad >> 1 & 1);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const h2v h0 = cvt2(x[0][e], x[1][e]), h1 = cvt2(x[2][e], x[3][e]);
-                    const int at = (4 * c + e) * VP + 4 * place;
-                    *reinterpret_cast<h4v *>(&lds.v[0][at]) = h4v{h0.x, h0.y, h1.x, h1.y};
-                    if constexpr (PL == 2) {
-                        const h2v l0 = rest2(x[0][e], x[1][e], h0), l1 = rest2(x[2][e], x[3][e], h1);
-                        *reinterpret_cast<h4v *>(&lds.v[PL - 1][at]) = h4v{l0.x, l0.y, l1.x, l1.y};
-                    }
-                }
-            }
-            if (b + 1 < b1) load(b + 1);
-            if (wave == 0) {
-                put_off(b + 2, pg);
-                pg = page_at(b + 3);
-            }
-            __syncthreads();
-            // scores
-            f16v s[2];
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = 0.0f;
+        if (tid < 4) lds.odd[tid] = 0;
+        // q: columns 16 ks + 8 half .. of the row, scaled, split
+        h8v qh[KS], ql[KS];
+        int qe;
+        {
+            f4v x[KS][2];
+            unsigned top = 0;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int kh = 0; kh < 2; kh++) {
-                    const int at = (kh * 32 + col) * KP + 16 * ks + 8 * half;
-                    const h8v h = *reinterpret_cast<const h8v *>(&lds.k[0][at]);
-                    s[kh] = mfma16(h, qh[ks], s[kh]);
-                    s[kh] = mfma16(h, ql[ks], s[kh]);
-                    if constexpr (PL == 2)
-                        s[kh] = mfma16(*reinterpret_cast<const h8v *>(&lds.k[PL - 1][at]), qh[ks], s[kh]);
+                for (int j = 0; j < 2; j++) {
+                    const int d = 16 * ks + 8 * half + 4 * j;
+                    x[ks][j] = f4v{0.f, 0.f, 0.f, 0.f};
+                    if (live && (!PAD || d < hd))
+                        x[ks][j] = *reinterpret_cast<const f4v *>(a.q + row * a.ldq + head * hd + d) * a.qscale;
+                    top = finite_top(top, x[ks][j]);
                 }
-            const float c = pow2(ke + qe);                   // scores are s * c
-            if (!lds.all[b & 3] || b * kUnit + kUnit > see0) {
+            const LanePair pr = pl32(__uint_as_float(top));
+            qe = max((int)(__float_as_uint(fmaxf(pr.lo, pr.hi)) >> 23) - 127, -100) - kTop;
+            const float sc = pow2(-qe);
 #pragma unroll
-                for (int kh = 0; kh < 2; kh++)
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int key = 32 * kh + 8 * (r >> 2) + 4 * half + (r & 3);
-                        if (lds.off[b & 3][key] < 0 || b * kUnit + key >= see) s[kh][r] = -INFINITY;
+                for (int j = 0; j < 2; j++) {
+                    h4v h, r;
+                    split4(x[ks][j] * sc, m1, h, r);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { qh[ks][4 * j + e] = h[e]; ql[ks][4 * j + e] = r[e]; }
+                }
+        }
+        __syncthreads();
+        // a unit's keys and values as they come: K thread (key, i): float4s i, i + KL, ..; V task (quad, c):
+        // keys 4 quad.., float4 c
+        typedef Raw4<BF16> RawK[KT], RawV[VT][4];
+        RawK rk;
+        RawV rv;
+        const int kkey = tid / KL, ki = tid % KL;
+        auto load = [&](int b, RawK &rk, RawV &rv) {
+            const long *off = lds.off[b & 3];
+            const bool all = lds.all[b & 3];
+            const long ko = off[kkey];
+#pragma unroll
+            for (int j = 0; j < KT; j++) {
+                const int i = ki + KL * j;
+                const bool in = !PAD || i < n4;
+                rk[j] = raw_load<BF16>(a.k, max(ko, 0l) + 4 * (in ? i : 0));
+                if (PAD && !in) rk[j] = raw_zero<BF16>();
+            }
+#pragma unroll
+            for (int t = 0; t < VT; t++) {
+                const int task = tid + t * NT, quad = min(task / C, 15), c = task % C;
+                const bool in = !PAD || c < n4;
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    rv[t][s] = raw_load<BF16>(a.v, max(off[4 * quad + s], 0l) + 4 * (in ? c : 0));
+                    if (PAD && !in) rv[t][s] = raw_zero<BF16>();
+                }
+            }
+            if (!all) {
+                if (ko < 0)
+#pragma unroll
+                    for (int j = 0; j < KT; j++) rk[j] = raw_zero<BF16>();
+#pragma unroll
+                for (int t = 0; t < VT; t++)
+#pragma unroll
+                    for (int s = 0; s < 4; s++)
+                        if (off[4 * min((tid + t * NT) / C, 15) + s] < 0) rv[t][s] = raw_zero<BF16>();
+            }
+        };
+        // its largest exponents, for all waves; values that are not finite leave it (the rows that see them get NaN)
+        auto tops = [&](int b, RawK &rk, RawV &rv) {
+            TopBits kb, vb;
+#pragma unroll
+            for (int j = 0; j < KT; j++) kb.add(widen(rk[j]));
+#pragma unroll
+            for (int t = 0; t < VT; t++)
+#pragma unroll
+                for (int s = 0; s < 4; s++) vb.add(widen(rv[t][s]));
+            u2v top = wave_top(top_halves(kb.bits(), vb.bits()));
+            if (top.x >= kNotFinite || top.y >= kNotFinite) {
+                if (top.y >= kNotFinite) {
+                    if (lane == 0) lds.odd[b & 3] = 1;
+#pragma unroll
+                    for (int t = 0; t < VT; t++)
+#pragma unroll
+                        for (int s = 0; s < 4; s++) drop_odd(rv[t][s]);
+                }
+                unsigned km = 0, vm = 0;
+#pragma unroll
+                for (int j = 0; j < KT; j++) km = finite_top(km, widen(rk[j]));
+#pragma unroll
+                for (int t = 0; t < VT; t++)
+#pragma unroll
+                    for (int s = 0; s < 4; s++) vm = finite_top(vm, widen(rv[t][s]));
+                top = wave_top(top_halves(km, vm));
+            }
+            if (lane == 0) lds.top[b & 1][wave] = __builtin_bit_cast(unsigned, top);
+        };
+        // exponents of the unit in LDS (k_e, v_e) and of the next; v_e only grows
+        int k_e = 0, v_e = -1000, k_n = 0, v_n = -1000;
+        auto next_exponents = [&](int b) {
+            u2v top = {0, 0};
+#pragma unroll
+            for (int w = 0; w < NW; w++) top = __builtin_elementwise_max(top, __builtin_bit_cast(u2v, lds.top[b & 1][w]));
+            k_n = max((int)(top.x >> 7) - 127, -100) - kTop;
+            v_n = max(v_e, max((int)(top.y >> 7) - 127, -100) - kTop);
+        };
+        auto split_unit = [&](int b, RawK &rk, RawV &rv) {
+            const float ks_ = pow2(-k_n), vs_ = pow2(-v_n);
+#pragma unroll
+            for (int j = 0; j < KT; j++) {
+                h4v h, r;
+                split4(widen(rk[j]) * ks_, m1, h, r);
+                const int at = kkey * KP + 4 * (ki + KL * j);
+                *reinterpret_cast<h4v *>(&lds.k[b & 1][0][at]) = h;
+                if constexpr (PL == 2) *reinterpret_cast<h4v *>(&lds.k[b & 1][PL - 1][at]) = r;
+            }
+#pragma unroll
+            for (int t = 0; t < VT; t++) {
+                const int task = tid + t * NT, quad = task / C, c = task % C;
+                f4v x[4];
+#pragma unroll
+                for (int s = 0; s < 4; s++) x[s] = widen(rv[t][s]) * vs_;
+                // quad 4 st + 2 b + h stands at place 4 st + 2 h + b
+                const int place = vplace(4 * c, (quad & ~3) | (quad & 1) << 1 | (quad >> 1 & 1));
+                if ((16 * C) % NT == 0 || quad < 16)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        h4v h, r;
+                        split4(f4v{x[0][e], x[1][e], x[2][e], x[3][e]}, m1, h, r);
+                        const int at = (4 * c + e) * VP + 4 * place;
+                        *reinterpret_cast<h4v *>(&lds.v[b & 1][0][at]) = h;
+                        if constexpr (PL == 2) *reinterpret_cast<h4v *>(&lds.v[b & 1][PL - 1][at]) = r;
                     }
             }
-            float top = fmaxf(s[0][0], s[1][0]);
+        };
+        f16v acc[DT];
 #pragma unroll
-            for (int r = 1; r < 16; r++) top = fmaxf(top, fmaxf(s[0][r], s[1][r]));
-            const LanePair pr = pl32(top);
-            top = fmaxf(pr.lo, pr.hi) * c;
-            // ve only grows; the accumulated values follow it, and m
-            if (__any(top > m + kLazy) || vnew != ve) {
-                const float mn = top > m + kLazy ? top : m;
-                const float f = exp2_hw(m - (mn == -INFINITY ? 0.0f : mn));
-                l *= f;
-                m = mn;
-                const float fv = f * (vnew - ve > 126 ? 0.0f : pow2(ve - vnew));
-                ve = vnew;
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int d = 0; d < DT; d++) acc[d] *= fv;
-            }
-            const float nm = (m == -INFINITY ? 0.0f : -m) + kBias;
-            float sum0 = 0.0f, sum1 = 0.0f;
+            for (int r = 0; r < 16; r++) acc[d][r] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+        int acc_e = -1000;                                   // acc counts in 2^acc_e
+        if (b0 < b1) {                                       // unit b0 to LDS, b0 + 1 to registers
+            RawK rk0;
+            RawV rv0;
+            load(b0, rk0, rv0);
+            load(b0 + 1, rk, rv);
+            tops(b0, rk0, rv0);
+            tops(b0 + 1, rk, rv);
+            __syncthreads();
+            next_exponents(b0);
+            split_unit(b0, rk0, rv0);
+            k_e = k_n;
+            v_e = v_n;
+            __syncthreads();
+        }
+        for (int b = b0; b < b1; b++) {
+            const bool odd = lds.odd[b & 3];
+            next_exponents(b + 1);
+            f16v s[2];
+            if (busy) {
 #pragma unroll
-            for (int kh = 0; kh < 2; kh++) {
+                for (int r = 0; r < 16; r++) s[0][r] = s[1][r] = 0.0f;
 #pragma unroll
-                for (int st = 0; st < 2; st++) {             // 16 keys
-                    h8v ph, pl;
+                for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float p0 = exp2_hw(fmaf(s[kh][8 * st + 2 * j], c, nm));
-                        const float p1 = exp2_hw(fmaf(s[kh][8 * st + 2 * j + 1], c, nm));
-                        sum0 += p0;
-                        sum1 += p1;
-                        const h2v h = cvt2(p0, p1), r = rest2(p0, p1, h);
-                        ph[2 * j] = h.x; ph[2 * j + 1] = h.y;
-                        pl[2 * j] = r.x; pl[2 * j + 1] = r.y;
-                    }
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        const int at = (32 * d + col) * VP + 4 * (8 * kh + 4 * st + 2 * half);
-                        const h8v h = *reinterpret_cast<const h8v *>(&lds.v[0][at]);
-                        acc[d] = mfma16(h, ph, acc[d]);
-                        acc[d] = mfma16(h, pl, acc[d]);
+                    for (int kh = 0; kh < 2; kh++) {
+                        const int at = (kh * 32 + col) * KP + 16 * ks + 8 * half;
+                        const h8v h = *reinterpret_cast<const h8v *>(&lds.k[b & 1][0][at]);
+                        s[kh] = mfma16(h, qh[ks], s[kh]);
+                        s[kh] = mfma16(h, ql[ks], s[kh]);
                         if constexpr (PL == 2)
-                            acc[d] = mfma16(*reinterpret_cast<const h8v *>(&lds.v[PL - 1][at]), ph, acc[d]);
+                            s[kh] = mfma16(*reinterpret_cast<const h8v *>(&lds.k[b & 1][PL - 1][at]), qh[ks], s[kh]);
                     }
-                }
+                split_unit(b + 1, rk, rv);
+            } else {
+                split_unit(b + 1, rk, rv);
             }
-            l += sum0 + sum1;
-            if (any_odd) {                                   // rows that see a value that is not finite
-                for (int key = 0; key < kUnit; key++) {
-                    const long off = lds.off[b & 3][key];
-                    if (off < 0 || b * kUnit + key >= see) continue;
-                    for (int d = 0; d < DT; d++)
+            load(b + 2, rk, rv);
+            if (((wave - b - 3) & (NW - 1)) == 0) {
+                put_off(b + 3, pg);
+                pg = page_at(b + 3 + NW);
+                if (lane == 0) lds.odd[(b + 3) & 3] = 0;
+            }
+            if (busy) {
+                const float c = pow2(k_e + qe);              // scores are s * c
+                if (!lds.all[b & 3] || b * kUnit + kUnit > see0) {
+#pragma unroll
+                    for (int kh = 0; kh < 2; kh++)
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
-                            const int at = 32 * d + 8 * (r >> 2) + 4 * half;
-                            if (at < hd && !finite_bits(widen(raw_load<BF16>(a.v, off + at))[r & 3])) acc[d][r] = NAN;
+                            const int key = 32 * kh + 8 * (r >> 2) + 4 * half + (r & 3);
+                            if (lds.off[b & 3][key] < 0 || b * kUnit + key >= see) s[kh][r] = -INFINITY;
                         }
                 }
+                float top = s[0][0];                         // (in a chain: two values an instruction)
+#pragma unroll
+                for (int r = 1; r < 32; r++) top = fmaxf(top, s[r >> 4][r & 15]);
+                const LanePair pr = pl32(top);
+                top = fmaxf(pr.lo, pr.hi) * c;
+                // the accumulated values follow m and v_e
+                if (__any(top > m + kLazy) || v_e != acc_e) {
+                    const float mn = top > m + kLazy ? top : m;
+                    const float f = exp2_hw(m - (mn == -INFINITY ? 0.0f : mn));
+                    l *= f;
+                    m = mn;
+                    const float fv = f * (v_e - acc_e > 126 ? 0.0f : pow2(acc_e - v_e));
+                    acc_e = v_e;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) acc[d] *= fv;
+                }
+                const float nm = (m == -INFINITY ? 0.0f : -m) + kBias;
+                float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                for (int kh = 0; kh < 2; kh++) {
+#pragma unroll
+                    for (int st = 0; st < 2; st++) {         // 16 keys
+                        h8v ph, pl;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float p0 = exp2_hw(fmaf(s[kh][8 * st + 2 * j], c, nm));
+                            const float p1 = exp2_hw(fmaf(s[kh][8 * st + 2 * j + 1], c, nm));
+                            sum0 += p0;
+                            sum1 += p1;
+                            h2v h, r;
+                            split2(p0, p1, m1, h, r);
+                            ph[2 * j] = h.x; ph[2 * j + 1] = h.y;
+                            pl[2 * j] = r.x; pl[2 * j + 1] = r.y;
+                        }
+#pragma unroll
+                        for (int d = 0; d < DT; d++) {
+                            const int at = (32 * d + col) * VP + 4 * vplace(32 * d + col, 8 * kh + 4 * st + 2 * half);
+                            const h8v h = *reinterpret_cast<const h8v *>(&lds.v[b & 1][0][at]);
+                            acc[d] = mfma16(h, ph, acc[d]);
+                            acc[d] = mfma16(h, pl, acc[d]);
+                            if constexpr (PL == 2)
+                                acc[d] = mfma16(*reinterpret_cast<const h8v *>(&lds.v[b & 1][PL - 1][at]), ph, acc[d]);
+                        }
+                    }
+                }
+                l += sum0 + sum1;
+                if (odd) {                                   // rows that see a value that is not finite
+                    for (int key = 0; key < kUnit; key++) {
+                        const long off = lds.off[b & 3][key];
+                        if (off < 0 || b * kUnit + key >= see) continue;
+#pragma unroll
+                        for (int d = 0; d < DT; d++)
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const int at = 32 * d + 8 * q + 4 * half;
+                                if (PAD && at >= hd) continue;
+                                const f4v x = widen(raw_load<BF16>(a.v, off + at));
+#pragma unroll
+                                for (int e = 0; e < 4; e++) acc[d][4 * q + e] = finite_bits(x[e]) ? acc[d][4 * q + e] : NAN;
+                            }
+                    }
+                }
             }
+            k_e = k_n;
+            v_e = v_n;
+            tops(b + 2, rk, rv);
+            __syncthreads();
         }
         {
             const LanePair pr = pl32(l);
             l = (pr.lo + pr.hi) * pow2(-kBias);
         }
-        const float unit = pow2(ve) * pow2(-kBias);          // what acc counts in
+        const float unit = pow2(acc_e) * pow2(-kBias);       // what acc counts in
         if (u == it.a && ue == it.b) {
             if (live) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -830,11 +902,11 @@ __global__ __launch_bounds__(kThreads, DT <= 2 ? 2 : 1) void k_attn_tile(AttnArg
                     for (int b = 0; b < 4; b++) {
                         const int at = 32 * d + 8 * b + 4 * half;
                         const f4v x = {acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]};
-                        if (at < hd) *reinterpret_cast<f4v *>(o + at) = x * unit * inv;
+                        if (!PAD || at < hd) *reinterpret_cast<f4v *>(o + at) = x * unit * inv;
                     }
             }
-        } else {
-            // [wave][4 d + b][lane] of float4, then (m, l) [wave][lane]
+        } else if (busy) {
+            // [wave][4 d + b][lane] of float4, then (m, l) of every row
             float *part = a.parts + (long)(2 * wg + (u == it.a)) * tile_part(DT);
             f4v *po = reinterpret_cast<f4v *>(part) + (long)wave * 4 * DT * 64 + lane;
 #pragma unroll
@@ -843,75 +915,126 @@ __global__ __launch_bounds__(kThreads, DT <= 2 ? 2 : 1) void k_attn_tile(AttnArg
                 for (int b = 0; b < 4; b++)
                     po[(4 * d + b) * 64] = f4v{acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]} * unit;
             if (half == 0)
-                *reinterpret_cast<f2v *>(part + kTileRows * 32 * DT + 2 * mrow) = f2v{m, l};
+                *reinterpret_cast<f2v *>(part + 32 * NW * 32 * DT + 2 * mrow) = f2v{m, l};
         }
         u = ue;
     }
 }
 
-template <int DT>
-__global__ __launch_bounds__(kThreads) void k_attn_tile_join(AttnArgs a, int n_wg) {
-    __shared__ Axis axis;
-    const int g = (int)blockIdx.x + 1, hd = a.hd, G = a.group.d;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
-    axis_init<true>(a, axis);
-    const Split split(axis.total, n_wg);
+// ── joining parts ────────────────────────────────────────────────────────
+// Boundary g of the n_wg stretches cuts an item, if no earlier boundary does:
+// its parts are those of workgroups g - 1 (slot 1) to last (slot 0).
+template <bool TILE>
+__device__ bool cut_item(const AttnArgs &a, Axis &x, int g, int n_wg, Item *it, int *last) {
+    const long total = axis_init<TILE>(a, x);
+    const Split split(total, n_wg);
     const long u = split.first(g);
-    if (u >= axis.total || u == 0) return;
-    const Item it = axis_item<true>(a, axis, u);
-    if (it.a >= u || split.first(g - 1) > it.a) return;
-    int last = g;
-    while (split.first(last + 1) < it.b) last++;
-    const int tt = a.tile_tokens, t0 = it.tile * tt;
-    const int mrow = wave * 32 + col, tok = t0 + a.group.quot(mrow), row = it.r.row0 + tok;
-    if (!(mrow < tt * G && tok < it.r.n && (unsigned)row < (unsigned)a.rows)) return;
-    const long head = it.kvh * G + mrow - (tok - t0) * G;
-    float m = -INFINITY, l = 0.0f;
-    f4v o[4 * DT];
-#pragma unroll
-    for (int i = 0; i < 4 * DT; i++) o[i] = f4v{0.f, 0.f, 0.f, 0.f};
-    for (int w = g - 1; w <= last; w++) {
-        const float *part = a.parts + (long)(2 * w + (w == g - 1)) * tile_part(DT);
-        const f4v *po = reinterpret_cast<const f4v *>(part) + (long)wave * 4 * DT * 64 + lane;
-        const f2v ml = *reinterpret_cast<const f2v *>(part + kTileRows * 32 * DT + 2 * mrow);
-        const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-        const float f = exp2_hw(m - ref), pf = exp2_hw(ml.x - ref);
-        l = l * f + ml.y * pf;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < 4 * DT; i++) o[i] = o[i] * f + po[i * 64] * pf;
+    if (u >= total || u == 0) return false;
+    *it = axis_item<TILE>(a, x, u);
+    if (it->a >= u || split.first(g - 1) > it->a) return false;
+    *last = g;
+    while (split.first(*last + 1) < it->b) ++*last;
+    return true;
+}
+
+// Blocks [0, n_few) take k_attn_few's boundaries, the others k_attn_tile's.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, int n_few, const float *tile_parts) {
+    constexpr int NW = tile_waves(DT), FR = kFewRows * few_pitch(DT);
+    __shared__ Axis axis;
+    Item it;
+    int last;
+    const int hd = a.hd, n4 = hd >> 2, G = a.group.d, tid = threadIdx.x;
+    if ((int)blockIdx.x < n_few) {
+        const int g = (int)blockIdx.x + 1;
+        if (!cut_item<false>(a, axis, g, n_few + 1, &it, &last)) return;
+        const int M = it.r.n * G;
+        for (int e = tid; e < M * n4; e += kThreads) {
+            const int i = e / n4, c = e - i * n4;
+            float m = -INFINITY, l = 0.0f;
+            f4v o = {0.f, 0.f, 0.f, 0.f};
+            for (int w = g - 1; w <= last; w++) {
+                const float *p = a.parts + (long)(2 * w + (w == g - 1)) * few_part(DT);
+                const f2v ml = *reinterpret_cast<const f2v *>(p + FR + 2 * i);
+                const f4v po = *reinterpret_cast<const f4v *>(p + i * few_pitch(DT) + 4 * c);
+                const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
+                const float f = exp2_hw(m - ref), pf = exp2_hw(ml.x - ref);
+                l = l * f + ml.y * pf;
+                o = o * f + po * pf;
+                m = mn;
+            }
+            const int t = a.group.quot(i), r = it.r.row0 + t;
+            if ((unsigned)r < (unsigned)a.rows)
+                *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(it.kvh * G + i - t * G) * hd + 4 * c) =
+                    o * (l == 0.0f ? 0.0f : 1.0f / l);
+        }
+        return;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float *out = a.out + row * a.ldo + head * hd;
+    const int g = (int)blockIdx.x - n_few + 1;
+    if (!cut_item<true>(a, axis, g, (int)gridDim.x - n_few + 1, &it, &last)) return;
+    const int tt = a.tile_tokens, t0 = it.tile * tt;
+    for (int e = tid; e < 64 * NW; e += kThreads) {          // as the lanes of the tile's waves
+        const int lane = e & 63, wave = e >> 6, half = lane >> 5, mrow = wave * 32 + (lane & 31);
+        const int tok = t0 + a.group.quot(mrow), row = it.r.row0 + tok;
+        if (!(mrow < tt * G && tok < it.r.n && (unsigned)row < (unsigned)a.rows)) continue;
+        float m = -INFINITY, l = 0.0f;
+        f4v o[4 * DT];
 #pragma unroll
-    for (int i = 0; i < 4 * DT; i++) {
-        const int at = 32 * (i >> 2) + 8 * (i & 3) + 4 * half;
-        if (at < hd) *reinterpret_cast<f4v *>(out + at) = o[i] * inv;
+        for (int i = 0; i < 4 * DT; i++) o[i] = f4v{0.f, 0.f, 0.f, 0.f};
+        for (int w = g - 1; w <= last; w++) {
+            const float *part = tile_parts + (long)(2 * w + (w == g - 1)) * tile_part(DT);
+            const f4v *po = reinterpret_cast<const f4v *>(part) + (long)wave * 4 * DT * 64 + lane;
+            const f2v ml = *reinterpret_cast<const f2v *>(part + 32 * NW * 32 * DT + 2 * mrow);
+            const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
+            const float f = exp2_hw(m - ref), pf = exp2_hw(ml.x - ref);
+            l = l * f + ml.y * pf;
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < 4 * DT; i++) o[i] = o[i] * f + po[i * 64] * pf;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        float *out = a.out + row * a.ldo + (it.kvh * G + mrow - (tok - t0) * G) * (long)hd;
+#pragma unroll
+        for (int i = 0; i < 4 * DT; i++) {
+            const int at = 32 * (i >> 2) + 8 * (i & 3) + 4 * half;
+            if (at < hd) *reinterpret_cast<f4v *>(out + at) = o[i] * inv;
+        }
     }
 }
 
 // ── launch ───────────────────────────────────────────────────────────────
-constexpr int kFewGroups = 1024, kTileGroups = 512;         // workgroups: what the chip holds at once
+constexpr int kFewGroups = 1024;                            // workgroups: what the chip holds at once
+constexpr int tile_groups(int dt) { return 2048 / tile_waves(dt); }
 
-int few_hq(int hd) { return hd <= 32 ? 2 : hd <= 64 ? 4 : hd <= 96 ? 6 : 8; }
 int tile_dt(int hd) { return (hd + 31) / 32; }
 
 typedef void (*Fn)(AttnArgs);
-typedef void (*JoinFn)(AttnArgs, int);
+typedef void (*JoinFn)(AttnArgs, int, const float *);
 
 template <int HQ>
 Fn few_fn(int hd, bool b16) {
     return hd == 16 * HQ ? (b16 ? k_attn_few<HQ, false, true> : k_attn_few<HQ, false, false>)
                          : (b16 ? k_attn_few<HQ, true, true> : k_attn_few<HQ, true, false>);
 }
+template <int DT>
+Fn tile_fn(int hd, bool b16) {
+    return hd == 32 * DT ? (b16 ? k_attn_tile<DT, false, true> : k_attn_tile<DT, false, false>)
+                         : (b16 ? k_attn_tile<DT, true, true> : k_attn_tile<DT, true, false>);
+}
 
-bool may_have_tiles(int group, int max_new) { return max_new == 0 || (long)max_new * group > kFewRows; }
-
-size_t work_floats(const ptmi_pages_t &p, int n_heads, int max_new, size_t *tile_at) {
-    size_t n = (size_t)2 * kFewGroups * few_part(few_hq(p.head_dim));
-    *tile_at = n;
-    if (may_have_tiles(n_heads / p.n_kv_heads, max_new)) n += (size_t)2 * kTileGroups * tile_part(tile_dt(p.head_dim));
-    return n;
+// Which kernels a call runs.
+struct Plan {
+    bool few, join_few, tile;
+    size_t tile_at, floats;          // of the workspace
+};
+Plan attn_plan(const ptmi_pages_t &p, int n_heads, int max_new) {
+    const int group = n_heads / p.n_kv_heads;
+    Plan c = {};
+    c.few = group <= kFewRows;
+    c.tile = max_new == 0 || (long)max_new * group > kFewRows;
+    c.floats = c.tile_at = c.few ? (size_t)2 * kFewGroups * few_part(tile_dt(p.head_dim)) : 0;
+    if (c.tile) c.floats += (size_t)2 * tile_groups(tile_dt(p.head_dim)) * tile_part(tile_dt(p.head_dim));
+    return c;
 }
 
 int check_heads(const char *who, const ptmi_pages_t *pages, int n_heads, int max_new) {
@@ -933,8 +1056,7 @@ extern "C" {
 
 size_t ptmi_paged_attention_work(const ptmi_pages_t *pages, int n_heads, int max_new) {
     if (check_heads("ptmi_paged_attention_work", pages, n_heads, max_new)) return 0;
-    size_t tile_at;
-    return work_floats(*pages, n_heads, max_new, &tile_at) * sizeof(float);
+    return attn_plan(*pages, n_heads, max_new).floats * sizeof(float);
 }
 
 int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, int table_width,
@@ -957,40 +1079,42 @@ int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, 
         return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: rows must be 16-byte aligned and hold %d heads (ldq=%ld ldo=%ld)",
                          n_heads, ldq, ldo);
     if (q == out) return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: out must not be q");
-    size_t tile_at;
-    const size_t need = work_floats(p, n_heads, max_new, &tile_at) * sizeof(float);
-    if (work_bytes < need)
-        return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: work holds %zu bytes, %zu needed", work_bytes, need);
+    const Plan plan = attn_plan(p, n_heads, max_new);
+    if (work_bytes < plan.floats * sizeof(float))
+        return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: work holds %zu bytes, %zu needed", work_bytes,
+                         plan.floats * sizeof(float));
     if ((st = ensure_init())) return st;
     DeviceScope dev;
     if ((st = dev.enter())) return st;
     const int group = n_heads / p.n_kv_heads;
     AttnArgs a = {p.k, p.v, p.page_stride, p.pos_stride, p.head_stride, p.n_pages, FastDiv(p.page_size), block_table,
                   table_width, row_start, kv_len, n_requests, q, ldq, out, ldo, rows, p.n_kv_heads, p.head_dim,
-                  FastDiv(group), kTileRows / group, scale * 1.44269504088896341f, (float *)work};
+                  FastDiv(group), 32 * tile_waves(tile_dt(p.head_dim)) / group, scale * 1.44269504088896341f,
+                  -1.0f, (float *)work};
     hipStream_t s = stream ? (hipStream_t)stream : lib_stream();
     const bool b16 = p.type == PTMI_BF16;
-    if (group <= kFewRows) {
-        const int hq = few_hq(p.head_dim);
-        const Fn fn = hq == 2 ? few_fn<2>(p.head_dim, b16) : hq == 4 ? few_fn<4>(p.head_dim, b16)
-                    : hq == 6 ? few_fn<6>(p.head_dim, b16) : few_fn<8>(p.head_dim, b16);
+    const int hd = p.head_dim;
+    const int dt = tile_dt(hd), n_tile = plan.tile ? tile_groups(dt) : 1;
+    if (plan.few) {
+        const Fn fn = dt == 1 ? few_fn<2>(hd, b16) : dt == 2 ? few_fn<4>(hd, b16) : dt == 3 ? few_fn<6>(hd, b16)
+                    : few_fn<8>(hd, b16);
         hipLaunchKernelGGL(fn, dim3(kFewGroups), dim3(kThreads), 0, s, a);
-        // no head has more than one unit: nothing to join
-        if ((long)table_width * p.page_size > kUnit)
-            hipLaunchKernelGGL(hq <= 4 ? k_attn_few_join<4> : k_attn_few_join<8>, dim3(kFewGroups - 1), dim3(kThreads), 0,
-                               s, a, kFewGroups);
-        PTMI_HIP(hipGetLastError());
     }
-    if (may_have_tiles(group, max_new)) {
-        a.parts = (float *)work + tile_at;
-        static const Fn fns[4][2] = {{k_attn_tile<1, false>, k_attn_tile<1, true>}, {k_attn_tile<2, false>, k_attn_tile<2, true>},
-                                     {k_attn_tile<3, false>, k_attn_tile<3, true>}, {k_attn_tile<4, false>, k_attn_tile<4, true>}};
-        static const JoinFn joins[4] = {k_attn_tile_join<1>, k_attn_tile_join<2>, k_attn_tile_join<3>, k_attn_tile_join<4>};
-        const int dt = tile_dt(p.head_dim);
-        hipLaunchKernelGGL(fns[dt - 1][b16], dim3(kTileGroups), dim3(kThreads), 0, s, a);
-        hipLaunchKernelGGL(joins[dt - 1], dim3(kTileGroups - 1), dim3(kThreads), 0, s, a, kTileGroups);
-        PTMI_HIP(hipGetLastError());
+    const float *tile_parts = a.parts + plan.tile_at;
+    if (plan.tile) {
+        const Fn fn = dt == 1 ? tile_fn<1>(hd, b16) : dt == 2 ? tile_fn<2>(hd, b16) : dt == 3 ? tile_fn<3>(hd, b16)
+                    : tile_fn<4>(hd, b16);
+        AttnArgs b = a;
+        b.parts += plan.tile_at;
+        hipLaunchKernelGGL(fn, dim3(n_tile), dim3(64 * tile_waves(dt)), 0, s, b);
     }
+    // One unit a head and nothing but single rows: nothing is ever cut.
+    if (plan.tile || (long)table_width * p.page_size > kUnit) {
+        const int n_few = plan.few ? kFewGroups - 1 : 0;
+        const JoinFn join = dt == 1 ? k_attn_join<1> : dt == 2 ? k_attn_join<2> : dt == 3 ? k_attn_join<3> : k_attn_join<4>;
+        hipLaunchKernelGGL(join, dim3(n_few + n_tile - 1), dim3(kThreads), 0, s, a, n_few, tile_parts);
+    }
+    PTMI_HIP(hipGetLastError());
     return PTMI_OK;
 }
 
