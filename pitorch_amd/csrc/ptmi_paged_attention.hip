@@ -36,6 +36,14 @@ constexpr int kFewRows = 16;         // rows of k_attn_few
 constexpr int kTileRows = 128;       // least rows of a tile of k_attn_tile
 constexpr int kThreads = 256;
 
+// An item whose units several workgroups take: its first part is slot 1 of
+// the workgroup it begins in, the others slot 0 of the next ones.
+struct Cut {
+    int parts;                       // 0: none
+    int row0, n, kvh, tile;
+    int pad[3];
+};
+
 struct AttnArgs {
     const void *k, *v;
     long page_stride, pos_stride, head_stride;
@@ -48,9 +56,11 @@ struct AttnArgs {
     int rows, kv_heads, hd;
     FastDiv group;                   // query heads of a key head
     int tile_tokens;                 // tokens of a tile: those whose rows it holds whole
+    int few_rows;                    // most rows of a request of the kernel for few
     float qscale;                    // scale * log2(e)
     float minus_one;
-    float *parts;                    // parts of heads cut between workgroups
+    float *parts;                    // parts of items cut between workgroups
+    Cut *cuts;                       // by workgroup: the cut item that begins in its stretch
 };
 
 // ── the axis of units ────────────────────────────────────────────────────
@@ -80,7 +90,7 @@ __device__ __forceinline__ long blocks_before(long k, long s, int tt) { return k
 
 template <bool TILE>
 __device__ __forceinline__ long head_units(const AttnArgs &a, const Request &r) {
-    const bool few = (long)r.n * a.group.d <= kFewRows;
+    const bool few = (long)r.n * a.group.d <= a.few_rows;
     if (r.n == 0 || few == TILE) return 0;
     if constexpr (TILE) {
         const int tt = a.tile_tokens, tiles = (r.n + tt - 1) / tt, k = tiles >> 6, rest = tiles & 63;
@@ -179,6 +189,10 @@ struct Split {
     long each, more;                 // the first `more` take each + 1
     __device__ Split(long total, int n) : each(quotient(total, n)), more(total - each * n) {}
     __device__ long first(int g) const { return g * each + min((long)g, more); }
+    __device__ int of(long u) const {                      // the workgroup that takes unit u
+        const long longer = more * (each + 1);
+        return (int)(u < longer ? quotient(u, each + 1) : more + quotient(u - longer, each));
+    }
 };
 
 // One item of the axis: a head's keys for one tile of rows, units [a, b).
@@ -211,6 +225,13 @@ __device__ Item axis_item(const AttnArgs &a, Axis &x, long u) {
         it.a = it.b - __shfl(mine, i) - tt * k;
     }
     return it;
+}
+
+// What a workgroup whose stretch ended in `it` tells k_attn_join.
+__device__ __forceinline__ void note_cut(const AttnArgs &a, int wg, const Split &split, const Item &it, long u, long ue) {
+    if (threadIdx.x) return;
+    const int parts = u == it.a && ue < it.b ? split.of(it.b - 1) - wg + 1 : 0;
+    a.cuts[wg] = Cut{parts, it.r.row0, it.r.n, it.kvh, it.tile, {0, 0, 0}};
 }
 
 // XCD x runs every eighth workgroup: give each XCD neighbouring stretches,
@@ -325,6 +346,7 @@ __global__ __launch_bounds__(kThreads) void k_attn_few(AttnArgs a) {
     const Split split(axis_init<false>(a, axis), gridDim.x);
     const int wg = stretch_of_block();
     const long u1 = split.first(wg + 1);
+    if (threadIdx.x == 0 && split.first(wg) == u1) a.cuts[wg].parts = 0;
     for (long u = split.first(wg); u < u1;) {
         const Item it = axis_item<false>(a, axis, u);
         const long ue = min(u1, it.b);
@@ -469,6 +491,240 @@ __global__ __launch_bounds__(kThreads) void k_attn_few(AttnArgs a) {
                 }
             }
         }
+        if (ue == u1) note_cut(a, wg, split, it, u, ue);
+        __syncthreads();
+        u = ue;
+    }
+}
+
+// ── one to four rows ─────────────────────────────────────────────────────
+// So few rows leave the matrix units' 16 idle; here the vector units do both
+// products.  Lane (g, li) of a wave takes keys 4g..4g+3 of 16 and float4s of
+// their rows: 16 lanes read a whole row of K or V side by side.  Scores are
+// summed over the 16 lanes; each lane group keeps a maximum and sums of its
+// own, and all 16 of the block's meet at the end.  64 requests of 12 heads x
+// 64, 180 MB of fp32: 55 us through the matrix instructions.
+constexpr float kLazyFew = 8.0f;     // a maximum up to 2^8 above m does not move m
+
+// FAST: four keys from a multiple of 4 on share a page, and bf16 rows may be
+// read 16 bytes at a time (page sizes of 4; head_dim and strides of 8).
+template <int C4, bool FAST, bool BF16>
+struct StreamBlock {                 // a lane's keys of 16
+    Raw4<BF16> k[4][C4], v[4][C4];
+    unsigned there;                  // bit s: key 4g + s is
+};
+
+// The float4 c of lane li's share of a row.
+template <int C4, bool BF16>
+__device__ __forceinline__ int stream_chunk(int li, int c) { return BF16 && C4 == 2 ? 2 * li + c : li + 16 * c; }
+
+template <int C4, bool FAST, bool BF16>
+__device__ __forceinline__ void stream_row(Raw4<BF16> (&r)[C4], const void *base, long at, int li, int n4) {
+    if constexpr (BF16 && C4 == 2 && FAST) {
+        const int i = min(2 * li, n4 - 2);
+        const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const unsigned short *>(base) + at + 4 * i);
+        r[0].x = make_uint2(x.x, x.y);
+        r[1].x = make_uint2(x.z, x.w);
+    } else {
+#pragma unroll
+        for (int c = 0; c < C4; c++) r[c] = raw_load<BF16>(base, at + 4 * min(stream_chunk<C4, BF16>(li, c), n4 - 1));
+    }
+}
+
+// Page numbers of the lane's keys (FAST: of the first).
+template <bool FAST>
+struct StreamPages { int pg[FAST ? 1 : 4]; };
+template <bool FAST>
+__device__ __forceinline__ StreamPages<FAST> stream_pages(const AttnArgs &a, int s, int key, int len) {
+    StreamPages<FAST> p;
+#pragma unroll
+    for (int i = 0; i < (FAST ? 1 : 4); i++) p.pg[i] = page_of(a, s, key + i, len);
+    return p;
+}
+
+template <int C4, bool FAST, bool BF16>
+__device__ __forceinline__ void stream_load(const AttnArgs &a, StreamBlock<C4, FAST, BF16> &b, int key, int len,
+                                            const StreamPages<FAST> &p, int kvh, int li, int n4) {
+    // keys that are not there read the cache's first row
+    const long first = key_offset(a, key, len, p.pg[0], kvh);
+    b.there = 0;
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+        long off;
+        if constexpr (FAST) off = first >= 0 && key + s < len ? first + s * a.pos_stride : -1;
+        else off = s == 0 ? first : key_offset(a, key + s, len, p.pg[FAST ? 0 : s], kvh);
+        if (off >= 0) b.there |= 1u << s;
+        off = max(off, 0l);
+        stream_row<C4, FAST, BF16>(b.k[s], a.k, off, li, n4);
+        stream_row<C4, FAST, BF16>(b.v[s], a.v, off, li, n4);
+    }
+}
+
+__device__ __forceinline__ float dot4(const f4v &x, const f4v &y, float s) {
+    return fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, s))));
+}
+
+template <int MR, int C4, bool FAST, bool BF16>
+__global__ __launch_bounds__(kThreads) void k_attn_stream(AttnArgs a) {
+    constexpr int NW = kThreads / 64, NP = 4 * NW, FP = few_pitch(2 * C4);
+    __shared__ Axis axis;
+    __shared__ __align__(16) float red[NP][MR][64 * C4];
+    __shared__ float st_m[NP][MR], st_l[NP][MR];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+    const int hd = a.hd, n4 = hd >> 2, G = a.group.d;
+    const Split split(axis_init<false>(a, axis), gridDim.x);
+    const int wg = stretch_of_block();
+    const long u1 = split.first(wg + 1);
+    if (threadIdx.x == 0 && split.first(wg) == u1) a.cuts[wg].parts = 0;
+    for (long u = split.first(wg); u < u1;) {
+        const Item it = axis_item<false>(a, axis, u);
+        const long ue = min(u1, it.b);
+        const int M = it.r.n * G, len = it.r.len;
+        int kb = (int)(u - it.a) * 4 + wave;
+        const int kend = (int)(ue - it.a) * 4;
+        StreamPages<FAST> pg = stream_pages<FAST>(a, it.s, kb * 16 + 4 * g, len);
+        f4v q[MR][C4];
+        int see[MR];
+#pragma unroll
+        for (int i = 0; i < MR; i++) {
+            const int tok = a.group.quot(i), row = it.r.row0 + tok;
+            see[i] = len - it.r.n + tok + 1;
+#pragma unroll
+            for (int c = 0; c < C4; c++) {
+                const int at = stream_chunk<C4, BF16>(li, c);
+                q[i][c] = f4v{0.f, 0.f, 0.f, 0.f};
+                if (i < M && (unsigned)row < (unsigned)a.rows && at < n4)
+                    q[i][c] = *reinterpret_cast<const f4v *>(a.q + row * a.ldq + (long)(it.kvh * G + i - tok * G) * hd + 4 * at) *
+                              a.qscale;
+            }
+        }
+        f4v acc[MR][C4];
+        float m[MR], l[MR];
+#pragma unroll
+        for (int i = 0; i < MR; i++) {
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < C4; c++) acc[i][c] = f4v{0.f, 0.f, 0.f, 0.f};
+        }
+        StreamBlock<C4, FAST, BF16> cur, nxt;
+        stream_load(a, cur, kb * 16 + 4 * g, len, pg, it.kvh, li, n4);
+        pg = stream_pages<FAST>(a, it.s, (kb + NW) * 16 + 4 * g, len);
+        for (; kb < kend; kb += NW) {
+            stream_load(a, nxt, (kb + NW) * 16 + 4 * g, kb + NW < kend ? len : 0, pg, it.kvh, li, n4);
+            pg = stream_pages<FAST>(a, it.s, (kb + 2 * NW) * 16 + 4 * g, len);
+            float s[MR][4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                f4v x[C4];
+#pragma unroll
+                for (int c = 0; c < C4; c++) x[c] = widen(cur.k[t][c]);
+#pragma unroll
+                for (int i = 0; i < MR; i++) {
+                    float d = dot4(x[0], q[i][0], 0.0f);
+                    if constexpr (C4 == 2) d = dot4(x[1], q[i][1], d);
+                    s[i][t] = group_sum<16>(d);
+                }
+            }
+            const int key = kb * 16 + 4 * g;
+            // every row sees all 16 keys
+            const bool full = __all(cur.there == 15u) && kb * 16 + 16 <= see[0];
+            if (!full) {
+#pragma unroll
+                for (int i = 0; i < MR; i++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+                        if (!(cur.there >> t & 1) || key + t >= see[i]) s[i][t] = -INFINITY;
+            }
+            bool move = false;
+#pragma unroll
+            for (int i = 0; i < MR; i++) move |= fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])) > m[i] + kLazyFew;
+            if (__any(move)) {
+#pragma unroll
+                for (int i = 0; i < MR; i++) {
+                    const float mn = fmaxf(m[i], fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
+                    const float f = exp2_hw(m[i] - (mn == -INFINITY ? 0.0f : mn));
+                    m[i] = mn;
+                    l[i] *= f;
+#pragma unroll
+                    for (int c = 0; c < C4; c++) acc[i][c] *= f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MR; i++) {
+                const float ref = m[i] == -INFINITY ? 0.0f : m[i];
+#pragma unroll
+                for (int t = 0; t < 4; t++) s[i][t] = exp2_hw(s[i][t] - ref);
+                l[i] += (s[i][0] + s[i][1]) + (s[i][2] + s[i][3]);
+            }
+            if (full) {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int c = 0; c < C4; c++) {
+                        const f4v v = widen(cur.v[t][c]);
+#pragma unroll
+                        for (int i = 0; i < MR; i++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[i][c][e] = fmaf(s[i][t], v[e], acc[i][c][e]);
+                    }
+            } else {                                         // an unseen value may be a NaN: it is not multiplied
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int c = 0; c < C4; c++) {
+                        const f4v v = widen(cur.v[t][c]);
+#pragma unroll
+                        for (int i = 0; i < MR; i++)
+                            if ((cur.there >> t & 1) && key + t < see[i])
+#pragma unroll
+                                for (int e = 0; e < 4; e++) acc[i][c][e] = fmaf(s[i][t], v[e], acc[i][c][e]);
+                    }
+            }
+            cur = nxt;
+        }
+        const int part_i = 4 * wave + g;
+        if (li < MR) {
+            st_m[part_i][li] = MR == 1 ? m[0] : li == 0 ? m[0] : li == 1 ? m[1 % MR] : li == 2 ? m[2 % MR] : m[3 % MR];
+            st_l[part_i][li] = MR == 1 ? l[0] : li == 0 ? l[0] : li == 1 ? l[1 % MR] : li == 2 ? l[2 % MR] : l[3 % MR];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MR; i++) {
+            float gm = -INFINITY;
+#pragma unroll
+            for (int p = 0; p < NP; p++) gm = fmaxf(gm, st_m[p][i]);
+            const float f = exp2_hw(m[i] - (gm == -INFINITY ? 0.0f : gm));
+#pragma unroll
+            for (int c = 0; c < C4; c++)
+                *reinterpret_cast<f4v *>(&red[part_i][i][4 * stream_chunk<C4, BF16>(li, c)]) = acc[i][c] * f;
+        }
+        __syncthreads();
+        const bool whole = u == it.a && ue == it.b;
+        float *part = a.parts + (long)(2 * wg + (u == it.a)) * few_part(2 * C4);
+        for (int e = threadIdx.x; e < min(M, MR) * n4; e += kThreads) {
+            const int i = e / n4, c = e - i * n4;
+            float im = -INFINITY, il = 0.0f;
+#pragma unroll
+            for (int p = 0; p < NP; p++) im = fmaxf(im, st_m[p][i]);
+            const float iref = im == -INFINITY ? 0.0f : im;
+            f4v o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                o += *reinterpret_cast<const f4v *>(&red[p][i][4 * c]);
+                il += st_l[p][i] * exp2_hw(st_m[p][i] - iref);
+            }
+            if (whole) {
+                const int t = a.group.quot(i), r = it.r.row0 + t;
+                if ((unsigned)r < (unsigned)a.rows)
+                    *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(it.kvh * G + i - t * G) * hd + 4 * c) =
+                        o * (il == 0.0f ? 0.0f : 1.0f / il);
+            } else {
+                *reinterpret_cast<f4v *>(part + i * FP + 4 * c) = o;
+                if (c == 0) *reinterpret_cast<f2v *>(part + kFewRows * FP + 2 * i) = f2v{im, il};
+            }
+        }
+        if (ue == u1) note_cut(a, wg, split, it, u, ue);
         __syncthreads();
         u = ue;
     }
@@ -594,6 +850,7 @@ __global__ __launch_bounds__(64 * tile_waves(DT), 2) void k_attn_tile(AttnArgs a
     const Split split(axis_init<true>(a, axis), gridDim.x);
     const int wg = stretch_of_block();
     const long u1 = split.first(wg + 1);
+    if (threadIdx.x == 0 && split.first(wg) == u1) a.cuts[wg].parts = 0;
     for (long u = split.first(wg); u < u1;) {
         const Item it = axis_item<true>(a, axis, u);
         const long ue = min(u1, it.b);
@@ -917,104 +1174,123 @@ __global__ __launch_bounds__(64 * tile_waves(DT), 2) void k_attn_tile(AttnArgs a
             if (half == 0)
                 *reinterpret_cast<f2v *>(part + 32 * NW * 32 * DT + 2 * mrow) = f2v{m, l};
         }
+        if (ue == u1) note_cut(a, wg, split, it, u, ue);
         u = ue;
     }
 }
 
 // ── joining parts ────────────────────────────────────────────────────────
-// Boundary g of the n_wg stretches cuts an item, if no earlier boundary does:
-// its parts are those of workgroups g - 1 (slot 1) to last (slot 0).
-template <bool TILE>
-__device__ bool cut_item(const AttnArgs &a, Axis &x, int g, int n_wg, Item *it, int *last) {
-    const long total = axis_init<TILE>(a, x);
-    const Split split(total, n_wg);
-    const long u = split.first(g);
-    if (u >= total || u == 0) return false;
-    *it = axis_item<TILE>(a, x, u);
-    if (it->a >= u || split.first(g - 1) > it->a) return false;
-    *last = g;
-    while (split.first(*last + 1) < it->b) ++*last;
-    return true;
+// A running (m, l, o) over parts.
+struct Join {
+    float m, l;
+    f4v o;
+    __device__ __forceinline__ void add(float pm, float pl, const f4v &po) {
+        const float mn = fmaxf(m, pm), ref = mn == -INFINITY ? 0.0f : mn;
+        const float f = exp2_hw(m - ref), pf = exp2_hw(pm - ref);
+        l = l * f + pl * pf;
+        o = o * f + po * pf;
+        m = mn;
+    }
+};
+// Adds parts first, first + step, .. < n, AHEAD of them on their way at once: their (m, l) `ml` floats and their
+// values `at` floats into each.
+template <int AHEAD, typename F>
+__device__ __forceinline__ void join_parts(Join &j, int first, int step, int n, long ml, long at, F &&part_of) {
+    for (int p0 = first; p0 < n; p0 += AHEAD * step) {
+        f2v pml[AHEAD];
+        f4v po[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const float *p = part_of(min(p0 + i * step, n - 1));
+            pml[i] = *reinterpret_cast<const f2v *>(p + ml);
+            po[i] = *reinterpret_cast<const f4v *>(p + at);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (p0 + i * step < n) j.add(pml[i].x, pml[i].y, po[i]);
+    }
 }
 
-// Blocks [0, n_few) take k_attn_few's boundaries, the others k_attn_tile's.
+// Block w joins the item that workgroup w of k_attn_few or k_attn_stream
+// noted; blocks from n_few on those of k_attn_tile.  Its threads share the
+// item's float4s and, where those are few, its parts.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, int n_few, const float *tile_parts) {
+__global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, int n_few, const Cut *tile_cuts, const float *tile_parts) {
     constexpr int NW = tile_waves(DT), FR = kFewRows * few_pitch(DT);
-    __shared__ Axis axis;
-    Item it;
-    int last;
+    __shared__ Join part[kThreads];
     const int hd = a.hd, n4 = hd >> 2, G = a.group.d, tid = threadIdx.x;
     if ((int)blockIdx.x < n_few) {
-        const int g = (int)blockIdx.x + 1;
-        if (!cut_item<false>(a, axis, g, n_few + 1, &it, &last)) return;
-        const int M = it.r.n * G;
-        for (int e = tid; e < M * n4; e += kThreads) {
-            const int i = e / n4, c = e - i * n4;
-            float m = -INFINITY, l = 0.0f;
-            f4v o = {0.f, 0.f, 0.f, 0.f};
-            for (int w = g - 1; w <= last; w++) {
-                const float *p = a.parts + (long)(2 * w + (w == g - 1)) * few_part(DT);
-                const f2v ml = *reinterpret_cast<const f2v *>(p + FR + 2 * i);
-                const f4v po = *reinterpret_cast<const f4v *>(p + i * few_pitch(DT) + 4 * c);
-                const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-                const float f = exp2_hw(m - ref), pf = exp2_hw(ml.x - ref);
-                l = l * f + ml.y * pf;
-                o = o * f + po * pf;
-                m = mn;
+        const int w = blockIdx.x;
+        const Cut c = a.cuts[w];
+        if (c.parts == 0) return;
+        auto part_of = [&](int p) { return a.parts + (long)(2 * (w + p) + (p == 0)) * few_part(DT); };
+        const int n = c.n * G * n4, slices = max(1, kThreads / n), lanes = min(n, kThreads);   // slices of parts
+        for (int e0 = 0; e0 < n; e0 += kThreads) {
+            const int e = e0 + tid % lanes, slice = tid / lanes, i = e / n4, col = e - i * n4;
+            Join j = {-INFINITY, 0.0f, {0.f, 0.f, 0.f, 0.f}};
+            if (e < n && slice < slices)
+                join_parts<8>(j, slice, slices, c.parts, FR + 2 * i, i * few_pitch(DT) + 4 * col, part_of);
+            part[tid] = j;
+            __syncthreads();
+            if (slice == 0 && e < n) {
+                for (int s = 1; s < slices; s++) {
+                    const Join &o = part[tid + s * lanes];
+                    j.add(o.m, o.l, o.o);
+                }
+                const int t = a.group.quot(i), r = c.row0 + t;
+                if ((unsigned)r < (unsigned)a.rows)
+                    *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(c.kvh * G + i - t * G) * hd + 4 * col) =
+                        j.o * (j.l == 0.0f ? 0.0f : 1.0f / j.l);
             }
-            const int t = a.group.quot(i), r = it.r.row0 + t;
-            if ((unsigned)r < (unsigned)a.rows)
-                *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(it.kvh * G + i - t * G) * hd + 4 * c) =
-                    o * (l == 0.0f ? 0.0f : 1.0f / l);
+            __syncthreads();
         }
         return;
     }
-    const int g = (int)blockIdx.x - n_few + 1;
-    if (!cut_item<true>(a, axis, g, (int)gridDim.x - n_few + 1, &it, &last)) return;
-    const int tt = a.tile_tokens, t0 = it.tile * tt;
-    for (int e = tid; e < 64 * NW; e += kThreads) {          // as the lanes of the tile's waves
-        const int lane = e & 63, wave = e >> 6, half = lane >> 5, mrow = wave * 32 + (lane & 31);
-        const int tok = t0 + a.group.quot(mrow), row = it.r.row0 + tok;
-        if (!(mrow < tt * G && tok < it.r.n && (unsigned)row < (unsigned)a.rows)) continue;
-        float m = -INFINITY, l = 0.0f;
-        f4v o[4 * DT];
-#pragma unroll
-        for (int i = 0; i < 4 * DT; i++) o[i] = f4v{0.f, 0.f, 0.f, 0.f};
-        for (int w = g - 1; w <= last; w++) {
-            const float *part = tile_parts + (long)(2 * w + (w == g - 1)) * tile_part(DT);
-            const f4v *po = reinterpret_cast<const f4v *>(part) + (long)wave * 4 * DT * 64 + lane;
-            const f2v ml = *reinterpret_cast<const f2v *>(part + 32 * NW * 32 * DT + 2 * mrow);
-            const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-            const float f = exp2_hw(m - ref), pf = exp2_hw(ml.x - ref);
-            l = l * f + ml.y * pf;
-            m = mn;
-#pragma unroll
-            for (int i = 0; i < 4 * DT; i++) o[i] = o[i] * f + po[i * 64] * pf;
-        }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        float *out = a.out + row * a.ldo + (it.kvh * G + mrow - (tok - t0) * G) * (long)hd;
-#pragma unroll
-        for (int i = 0; i < 4 * DT; i++) {
-            const int at = 32 * (i >> 2) + 8 * (i & 3) + 4 * half;
-            if (at < hd) *reinterpret_cast<f4v *>(out + at) = o[i] * inv;
-        }
+    // four blocks an item: float4 q of every fourth
+    const int w = ((int)blockIdx.x - n_few) >> 2, q0 = (int)blockIdx.x - n_few & 3;
+    const Cut c = tile_cuts[w];
+    if (c.parts == 0) return;
+    auto part_of = [&](int p) { return tile_parts + (long)(2 * (w + p) + (p == 0)) * tile_part(DT); };
+    const int tt = a.tile_tokens, t0 = c.tile * tt;
+    for (int e = tid; e < 64 * NW * DT; e += kThreads) {     // as the lanes of the tile's waves
+        const int lane = e & 63, wave = (e >> 6) % NW, q = 4 * (e / (64 * NW)) + q0;
+        const int mrow = wave * 32 + (lane & 31), at = 8 * q + 4 * (lane >> 5);
+        const int tok = t0 + a.group.quot(mrow), row = c.row0 + tok;
+        if (!(mrow < tt * G && tok < c.n && (unsigned)row < (unsigned)a.rows && at < hd)) continue;
+        Join j = {-INFINITY, 0.0f, {0.f, 0.f, 0.f, 0.f}};
+        join_parts<2>(j, 0, 1, c.parts, 32 * NW * 32 * DT + 2 * mrow, 4l * ((wave * 4 * DT + q) * 64 + lane), part_of);
+        *reinterpret_cast<f4v *>(a.out + row * a.ldo + (c.kvh * G + mrow - (tok - t0) * G) * (long)hd + at) =
+            j.o * (j.l == 0.0f ? 0.0f : 1.0f / j.l);
     }
 }
 
 // ── launch ───────────────────────────────────────────────────────────────
 constexpr int kFewGroups = 1024;                            // workgroups: what the chip holds at once
+constexpr int kTileGroups = 512;
 constexpr int tile_groups(int dt) { return 2048 / tile_waves(dt); }
 
 int tile_dt(int hd) { return (hd + 31) / 32; }
 
 typedef void (*Fn)(AttnArgs);
-typedef void (*JoinFn)(AttnArgs, int, const float *);
+typedef void (*JoinFn)(AttnArgs, int, const Cut *, const float *);
 
 template <int HQ>
 Fn few_fn(int hd, bool b16) {
     return hd == 16 * HQ ? (b16 ? k_attn_few<HQ, false, true> : k_attn_few<HQ, false, false>)
                          : (b16 ? k_attn_few<HQ, true, true> : k_attn_few<HQ, true, false>);
+}
+template <int MR, int C4>
+Fn stream_fn2(bool fast, bool b16) {
+    return fast ? (b16 ? k_attn_stream<MR, C4, true, true> : k_attn_stream<MR, C4, true, false>)
+                : (b16 ? k_attn_stream<MR, C4, false, true> : k_attn_stream<MR, C4, false, false>);
+}
+Fn stream_fn(int rows, const ptmi_pages_t &p) {
+    const bool b16 = p.type == PTMI_BF16, wide = p.head_dim > 64;
+    const bool fast = p.page_size % 4 == 0 &&
+                      !(b16 && (p.head_dim | p.page_stride | p.pos_stride | p.head_stride) % 8);
+    return rows == 1 ? (wide ? stream_fn2<1, 2>(fast, b16) : stream_fn2<1, 1>(fast, b16))
+         : rows == 2 ? (wide ? stream_fn2<2, 2>(fast, b16) : stream_fn2<2, 1>(fast, b16))
+                     : (wide ? stream_fn2<4, 2>(fast, b16) : stream_fn2<4, 1>(fast, b16));
 }
 template <int DT>
 Fn tile_fn(int hd, bool b16) {
@@ -1024,15 +1300,20 @@ Fn tile_fn(int hd, bool b16) {
 
 // Which kernels a call runs.
 struct Plan {
-    bool few, join_few, tile;
-    size_t tile_at, floats;          // of the workspace
+    bool few, tile;
+    int stream;                      // rows of k_attn_stream in k_attn_few's place; 0: not
+    size_t few_at, tile_at, floats;  // of the workspace (the cuts come first)
 };
 Plan attn_plan(const ptmi_pages_t &p, int n_heads, int max_new) {
     const int group = n_heads / p.n_kv_heads;
     Plan c = {};
     c.few = group <= kFewRows;
     c.tile = max_new == 0 || (long)max_new * group > kFewRows;
-    c.floats = c.tile_at = c.few ? (size_t)2 * kFewGroups * few_part(tile_dt(p.head_dim)) : 0;
+    if (max_new > 0 && (long)max_new * group <= 4) c.stream = max_new * group == 3 ? 4 : max_new * group;
+    c.tile_at = (kFewGroups + kTileGroups) * sizeof(Cut) / sizeof(float);
+    c.few_at = c.tile_at;
+    c.tile_at += c.few ? (size_t)2 * kFewGroups * few_part(tile_dt(p.head_dim)) : 0;
+    c.floats = c.tile_at;
     if (c.tile) c.floats += (size_t)2 * tile_groups(tile_dt(p.head_dim)) * tile_part(tile_dt(p.head_dim));
     return c;
 }
@@ -1089,30 +1370,33 @@ int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, 
     const int group = n_heads / p.n_kv_heads;
     AttnArgs a = {p.k, p.v, p.page_stride, p.pos_stride, p.head_stride, p.n_pages, FastDiv(p.page_size), block_table,
                   table_width, row_start, kv_len, n_requests, q, ldq, out, ldo, rows, p.n_kv_heads, p.head_dim,
-                  FastDiv(group), 32 * tile_waves(tile_dt(p.head_dim)) / group, scale * 1.44269504088896341f,
-                  -1.0f, (float *)work};
+                  FastDiv(group), 32 * tile_waves(tile_dt(p.head_dim)) / group, plan.stream ? plan.stream : kFewRows,
+                  scale * 1.44269504088896341f,
+                  -1.0f, (float *)work + plan.few_at, (Cut *)work};
     hipStream_t s = stream ? (hipStream_t)stream : lib_stream();
     const bool b16 = p.type == PTMI_BF16;
     const int hd = p.head_dim;
     const int dt = tile_dt(hd), n_tile = plan.tile ? tile_groups(dt) : 1;
     if (plan.few) {
-        const Fn fn = dt == 1 ? few_fn<2>(hd, b16) : dt == 2 ? few_fn<4>(hd, b16) : dt == 3 ? few_fn<6>(hd, b16)
+        const Fn fn = plan.stream ? stream_fn(plan.stream, p) : dt == 1 ? few_fn<2>(hd, b16) : dt == 2 ? few_fn<4>(hd, b16) : dt == 3 ? few_fn<6>(hd, b16)
                     : few_fn<8>(hd, b16);
         hipLaunchKernelGGL(fn, dim3(kFewGroups), dim3(kThreads), 0, s, a);
     }
-    const float *tile_parts = a.parts + plan.tile_at;
     if (plan.tile) {
         const Fn fn = dt == 1 ? tile_fn<1>(hd, b16) : dt == 2 ? tile_fn<2>(hd, b16) : dt == 3 ? tile_fn<3>(hd, b16)
                     : tile_fn<4>(hd, b16);
         AttnArgs b = a;
-        b.parts += plan.tile_at;
+        b.parts = (float *)work + plan.tile_at;
+        b.cuts = a.cuts + kFewGroups;
         hipLaunchKernelGGL(fn, dim3(n_tile), dim3(64 * tile_waves(dt)), 0, s, b);
     }
     // One unit a head and nothing but single rows: nothing is ever cut.
     if (plan.tile || (long)table_width * p.page_size > kUnit) {
-        const int n_few = plan.few ? kFewGroups - 1 : 0;
+        // (the last workgroup's stretch ends with an item)
+        const int n_few = plan.few ? kFewGroups - 1 : 0, n_join = plan.tile ? 4 * (n_tile - 1) : 0;
         const JoinFn join = dt == 1 ? k_attn_join<1> : dt == 2 ? k_attn_join<2> : dt == 3 ? k_attn_join<3> : k_attn_join<4>;
-        hipLaunchKernelGGL(join, dim3(n_few + n_tile - 1), dim3(kThreads), 0, s, a, n_few, tile_parts);
+        hipLaunchKernelGGL(join, dim3(n_few + n_join), dim3(kThreads), 0, s, a, n_few, a.cuts + kFewGroups,
+                           (const float *)work + plan.tile_at);
     }
     PTMI_HIP(hipGetLastError());
     return PTMI_OK;
