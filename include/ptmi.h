@@ -383,8 +383,9 @@ size_t ptmi_paged_attention_work(const ptmi_pages_t *pages, int n_heads, int max
  * order of indices, exceeds u times its whole (u clamped to [0, 1)).
  * temperature <= 0 (or NaN): the first index of the maximum.  NaN logits
  * count as -infinity, and with nothing above that the token is -1; among
- * infinite maxima only they stay.  w below 2^-45 counts as 0.  Sums are
- * integers of 2^-44: a row's result depends on nothing else.             */
+ * infinite maxima only they stay.  w is held as a multiple of 2^-44 (at most
+ * 0.9 of it off) and added up exactly: a row's token depends on nothing but
+ * the row and its parameters.  vocab: at most 262140.                    */
 int ptmi_sample_dev(const float *logits, long ld, int rows, int vocab, const float *temperature, const int *top_k,
                     const float *top_p, const float *min_p, const float *u, int *token, void *stream);
 

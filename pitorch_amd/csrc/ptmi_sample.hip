@@ -1,21 +1,34 @@
-// Sampling of one token per row of logits.
+// Sampling of one token per row of logits: one workgroup a row.
 //
-// A row's order is that of its keys: the logits' bits made monotone, larger
-// logits first, equal ones by index.  Every filter keeps a beginning of that
-// order, so what stays is known by one (key, number of that key's logits):
-// found by rounds over the key's bits, each a histogram of what shares the
-// bits found so far, of counts for top_k and of weights for top_p.  Weights
-// are whole multiples of 2^-44 in 64 bits: their sums are exact and the same
-// in any order, so shared-memory atomics leave the result unchanged.
+// A row's order is that of its logits, larger first, equal ones by index, and
+// every filter keeps a beginning of it: what stays is known by the smallest
+// logit that stays and how many of its equals do.  top_k looks for the logit
+// at which a count, top_p for the one at which a sum of weights reaches its
+// mark: a histogram of the logits between two bounds in kBins bins of equal
+// width, the bin that holds the mark, and so on in that bin; once few enough
+// logits are left in it they are compared with each other.  A step is two
+// passes over the row (one that fills the bins, one that takes out the
+// members of the bin found), and of a language model's logits one step is
+// enough.  The row is read from memory once, into shared memory (up to 32768
+// logits; longer rows are read again, from the caches, for every pass).
+//
+// Weights are whole multiples of 2^-44 in 64 bits: sums of them are exact and
+// the same in any order, so the atomics of the bins leave the result as it is.
 #include "ptmi_paged.h"
+
+#include <cfloat>
 
 namespace ptmi {
 
 namespace {
 
 typedef unsigned long long u64;
+typedef float f4v __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kBins = 2 * kThreads;
+constexpr int kList = 128;           // logits of a bin that are compared with each other
+constexpr int kMaxVocab = (1 << 18) - 4;                    // 64 turns of a block, wherever in a float4 a row starts
 
 struct SampleArgs {
     const float *logits; long ld;
@@ -24,175 +37,365 @@ struct SampleArgs {
     int *token;
 };
 
-// Larger key = larger logit; 0 for NaN and -infinity (never chosen).
-__device__ __forceinline__ unsigned key_of(float x) {
-    if (!(x > -INFINITY)) return 0u;
-    const unsigned b = __float_as_uint(x + 0.0f);           // -0 as 0
+// ── weights ──────────────────────────────────────────────────────────────
+// 2^y for y <= 0, 0 below -46: 2^n p(f), |f| <= 1/2, p of degree 9 through
+// 2^f at the Chebyshev nodes (relative error 1.9e-14, a third of 2^-44).
+__device__ __forceinline__ double exp2_weight(double y) {
+    const double n = __builtin_rint(y), f = y - n;
+    double p = 1.0205905413765595e-07;
+    p = fma(p, f, 1.325964524488711e-06);
+    p = fma(p, f, 1.5252672924850737e-05);
+    p = fma(p, f, 0.0001540343375125101);
+    p = fma(p, f, 0.0013333558200794592);
+    p = fma(p, f, 0.009618129193934313);
+    p = fma(p, f, 0.05550410866465167);
+    p = fma(p, f, 0.2402265069564034);
+    p = fma(p, f, 0.6931471805599462);
+    p = fma(p, f, 1.0000000000000135);
+    return y < -46.0 ? 0.0 : ldexp(p, (int)n);
+}
+// To the nearest multiple of 2^-44, as their number: w + 2^8 has them as its last bits.
+__device__ __forceinline__ u64 fixed(double w) {
+    return (u64)(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0));
+}
+
+// What a search adds up: counts, or weights.
+struct CountOf {
+    __device__ __forceinline__ u64 operator()(float) const { return 1; }
+};
+struct WeightOf {
+    float top;
+    double scale, min_p;             // log2(e) / temperature
+    __device__ __forceinline__ u64 operator()(float x) const {
+        const double w = x == top ? 1.0 : exp2_weight(((double)x - (double)top) * scale);
+        return w >= min_p ? fixed(w) : 0;
+    }
+};
+
+// ── sums over waves and the block ────────────────────────────────────────
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_add(u64 v) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xF, false);
+    return v + ((u64)hi << 32 | lo);
+}
+__device__ __forceinline__ u64 wave_scan(u64 v) {          // inclusive
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    return dpp_add<0x143, 0xC>(v);
+}
+
+struct SampleLds {
+    u64 bins[kBins];
+    u64 wave[kWaves];
+    float list_x[kList];
+    u64 list_w[kList];
+    unsigned lo, hi;                 // of a bin's members, as ordered bits
+    int members, bin, index;
+    u64 before, sum;
+    float value;
+    u64 block_sum[kThreads];         // sums of 256 consecutive logits' weights
+};
+
+// Floats as integers in the same order (-0 below 0).
+__device__ __forceinline__ unsigned ordered(float x) {
+    const unsigned b = __float_as_uint(x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float logit_of(unsigned k) {
+__device__ __forceinline__ float from_ordered(unsigned k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-struct Row { float top; double inv_t; };
-
-__device__ __forceinline__ double weight(const Row &r, float x) {
-    if (x == r.top) return 1.0;
-    return exp(((double)x - (double)r.top) * r.inv_t);
+// Inclusive sums over the block.
+__device__ __forceinline__ u64 block_scan(u64 v, SampleLds &s) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    v = wave_scan(v);
+    if (lane == 63) s.wave[w] = v;
+    __syncthreads();
+    for (int i = 0; i < w; i++) v += s.wave[i];
+    __syncthreads();
+    return v;
 }
-__device__ __forceinline__ u64 fixed(double w) { return (u64)(w * 17592186044416.0 + 0.5); }   // 2^44
 
-__global__ __launch_bounds__(kThreads) void k_sample_simple(SampleArgs a) {
-    __shared__ u64 hist[256], part[kThreads];
-    __shared__ unsigned red_k;
-    __shared__ int red_i, s_bin;
-    __shared__ u64 s_before;
-    const int t = threadIdx.x, V = a.vocab;
-    const float *x = a.logits + (long)blockIdx.x * a.ld;
-    auto row_f = [&](const float *p, float off) { return p ? p[blockIdx.x] : off; };
-    // the maximum and its first index
-    unsigned bk = 0;
-    for (int i = t; i < V; i += kThreads) bk = max(bk, key_of(x[i]));
-    if (t == 0) { red_k = 0; red_i = V; }
-    __syncthreads();
-    atomicMax(&red_k, bk);
-    __syncthreads();
-    const unsigned kmax = red_k;
-    const float temp = row_f(a.temperature, 1.0f);
-    if (kmax == 0) { if (t == 0) a.token[blockIdx.x] = -1; return; }
-    if (!(temp > 0.0f)) {
-        for (int i = t; i < V; i += kThreads)
-            if (key_of(x[i]) == kmax) { atomicMin(&red_i, i); break; }
-        __syncthreads();
-        if (t == 0) a.token[blockIdx.x] = red_i;
-        return;
+// ── a row ────────────────────────────────────────────────────────────────
+// The row's logits in float4s of 16 aligned bytes; in turn j thread t has
+// float4 t + 1024 j.  What stands before and behind the row in its first and
+// last float4 counts as -infinity, as NaN does; among infinite maxima only
+// they count, as 0.  LOCAL: `at` is a copy in shared memory, else the row.
+template <bool LOCAL>
+struct Row {
+    const f4v *at;
+    int skip, vocab, turns;          // floats before the row in its first float4; float4s of a thread
+    bool top_inf;
+
+    __device__ __forceinline__ int index(int j) const { return 4 * ((int)threadIdx.x + kThreads * j) - skip; }
+    __device__ __forceinline__ f4v fetch(int j) const {    // from memory
+        const int i = index(j);
+        f4v v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (i < vocab) {
+            v = at[threadIdx.x + kThreads * j];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[e] = (unsigned)(i + e) < (unsigned)vocab && v[e] > -INFINITY ? v[e] + 0.0f : -INFINITY;   // (-0 as 0)
+        }
+        return v;
     }
-    const Row row = {logit_of(kmax), 1.0 / (double)temp};
-    int top_k = a.top_k ? a.top_k[blockIdx.x] : 0;
-    const float top_p = row_f(a.top_p, 1.0f);
-    float mp = row_f(a.min_p, 0.0f);
-    const double min_p = mp > 1.0f ? 1.0 : mp > 0.0f ? (double)mp : 0.0;
-    float uf = row_f(a.u, 0.0f);
-    uf = uf > 0.0f ? fminf(uf, 0.99999994f) : 0.0f;
-    // kept: key > tk, and the first tn (by index) of key == tk
-    unsigned tk = 1;
-    int tn = V;
-    auto kept = [&](unsigned k) { return k >= tk; };
-    // the first key, from the largest down, at which the running sum of `measure` exceeds `target`:
-    // its key, and the sum before it
-    auto find = [&](auto measure, u64 target, unsigned *key, u64 *before) {
-        unsigned prefix = 0;
-        u64 sum = 0;
-        for (int sh = 24; sh >= 0; sh -= 8) {
-            for (int b = t; b < 256; b += kThreads) hist[b] = 0;
+    __device__ __forceinline__ f4v get(int j) const {
+        f4v v = LOCAL ? at[threadIdx.x + kThreads * j] : fetch(j);
+        if (top_inf)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = v[e] == INFINITY ? 0.0f : -INFINITY;
+        return v;
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F &&f) const {    // f(logit) for all of this thread's
+        for (int j = 0; j < turns; j++) {
+            const f4v v = get(j);
+#pragma unroll
+            for (int e = 0; e < 4; e++) f(v[e]);
+        }
+    }
+};
+
+// The logit at which the running sum of `measure` over the logits in [lo, hi],
+// in their order, reaches need(their whole sum), which is more than 0 and at
+// most that sum: its value, the sum before it and the sum of its equals.
+struct Mark { float value; u64 before, equals, need; };
+
+template <bool LOCAL, typename M, typename F>
+__device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float hi, const M &measure, F &&need_of) {
+    const int t = threadIdx.x;
+    Mark k = {hi, 0, 0, 0};
+    bool first = true;
+    for (;;) {
+        // lo < hi fall into different bins (but where they are equal), so the bounds close in
+        const double top = hi, inv = lo < hi ? kBins / (top - (double)lo) : 0.0;
+        auto bin_of = [&](float x) { return min((int)((top - (double)x) * inv), kBins - 1); };
+        s.bins[t] = s.bins[t + kThreads] = 0;
+        if (t == 0) { s.members = 0; s.lo = 0xFFFFFFFFu; s.hi = 0; }
+        __syncthreads();
+        row.each([&](float x) {
+            if (x >= lo && x <= hi) {
+                const u64 w = measure(x);
+                if (w) atomicAdd(&s.bins[bin_of(x)], w);
+            }
+        });
+        __syncthreads();
+        const u64 b0 = s.bins[2 * t], b1 = s.bins[2 * t + 1], c1 = block_scan(b0 + b1, s), c0 = c1 - b1, cb = c0 - b0;
+        if (first) {
+            if (t == kThreads - 1) s.before = c1;
             __syncthreads();
-            for (int i = t; i < V; i += kThreads) {
-                const unsigned k = key_of(x[i]);
-                if (k && kept(k) && (sh == 24 || k >> (sh + 8) == prefix)) {
-                    const u64 w = measure(i, k);
-                    if (w) atomicAdd(&hist[k >> sh & 255], w);
+            k.need = need_of(s.before);
+            __syncthreads();
+            first = false;
+        }
+        if (k.before + cb < k.need && k.need <= k.before + c0) { s.bin = 2 * t; s.before = k.before + cb; s.sum = b0; }
+        if (k.before + c0 < k.need && k.need <= k.before + c1) { s.bin = 2 * t + 1; s.before = k.before + c0; s.sum = b1; }
+        __syncthreads();
+        const int bin = s.bin;
+        k.before = s.before;
+        k.equals = s.sum;
+        k.value = hi;
+        if (!(lo < hi)) { __syncthreads(); return k; }      // all equal
+        float least = INFINITY, most = -INFINITY;
+        row.each([&](float x) {
+            if (x >= lo && x <= hi && bin_of(x) == bin) {
+                least = fminf(least, x);
+                most = fmaxf(most, x);
+                // (the count stops a little above kList)
+                if (*(volatile int *)&s.members <= kList) {
+                    const int at = atomicAdd(&s.members, 1);
+                    if (at < kList) { s.list_x[at] = x; s.list_w[at] = measure(x); }
                 }
             }
-            __syncthreads();
-            if (t == 0) {
-                int b = 255;
-                u64 c = sum;
-                while (b > 0 && c + hist[b] <= target) c += hist[b--];
-                s_bin = b;
-                s_before = c;
+        });
+        least = -group_max<64>(-least);
+        most = group_max<64>(most);
+        if ((t & 63) == 0 && least <= most) {
+            atomicMin(&s.lo, ordered(least));
+            atomicMax(&s.hi, ordered(most));
+        }
+        __syncthreads();
+        const int n = s.members;
+        lo = from_ordered(s.lo);
+        hi = from_ordered(s.hi);
+        if (n <= kList) {
+            if (t < n) {
+                const float x = s.list_x[t];
+                u64 above = k.before, equal = 0;
+                for (int i = 0; i < n; i++) {
+                    const float y = s.list_x[i];
+                    const u64 w = s.list_w[i];
+                    above += y > x ? w : 0;
+                    equal += y == x ? w : 0;
+                }
+                if (above < k.need && k.need <= above + equal) { s.value = x; s.before = above; s.sum = equal; }   // equals agree
             }
             __syncthreads();
-            prefix = prefix << 8 | (unsigned)s_bin;
-            sum = s_before;
+            k.value = s.value;
+            k.before = s.before;
+            k.equals = s.sum;
             __syncthreads();
+            return k;
         }
-        *key = prefix;
-        *before = sum;
-    };
-    if (top_k > 0 && top_k < V) {
-        unsigned key;
-        u64 before;
-        find([&](int, unsigned) -> u64 { return 1; }, (u64)(top_k - 1), &key, &before);
-        if (key > 0) { tk = key; tn = top_k - (int)before; }
+        __syncthreads();
     }
-    // index order: the weight of i as it stays (ties of tk only the first tn)
-    auto sum_all = [&](u64 w) -> u64 {                      // over the block
-        part[t] = w;
+}
+
+// CAP: logits that the copy in shared memory holds; 0: no copy.
+template <int CAP>
+__global__ __launch_bounds__(kThreads) void k_sample(SampleArgs a) {
+    __shared__ SampleLds s;
+    __shared__ f4v copy[CAP ? CAP / 4 : 1];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = blockIdx.x;
+    const float *logits = a.logits + (long)r * a.ld;
+    Row<(CAP > 0)> row;
+    row.skip = (int)((uintptr_t)logits >> 2 & 3);
+    row.at = reinterpret_cast<const f4v *>(logits - row.skip);
+    row.vocab = a.vocab;
+    row.turns = (a.vocab + row.skip + 4 * kThreads - 1) / (4 * kThreads);
+    row.top_inf = false;
+    const float temp = a.temperature ? a.temperature[r] : 1.0f;
+    const int top_k = a.top_k ? a.top_k[r] : 0;
+    const float top_p = a.top_p ? a.top_p[r] : 1.0f, min_pf = a.min_p ? a.min_p[r] : 0.0f;
+    float u = a.u ? a.u[r] : 0.0f;
+    // the largest logit
+    float top = -INFINITY;
+#pragma unroll 8
+    for (int j = 0; j < row.turns; j++) {
+        const f4v v = row.fetch(j);
+        if constexpr (CAP > 0) copy[t + kThreads * j] = v;   // (each thread reads back its own)
+        top = fmaxf(fmaxf(top, fmaxf(v[0], v[1])), fmaxf(v[2], v[3]));
+    }
+    if constexpr (CAP > 0) row.at = copy;
+    top = group_max<64>(top);
+    if (lane == 0) s.list_x[wave] = top;
+    if (t == 0) s.index = a.vocab;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) top = fmaxf(top, s.list_x[w]);
+    __syncthreads();
+    if (top == -INFINITY) {
+        if (t == 0) a.token[r] = -1;
+        return;
+    }
+    if (top == INFINITY) {                                   // uniform
+        row.top_inf = true;
+        top = 0.0f;
+    }
+    if (!(temp > 0.0f) || top_k == 1) {                      // the first index of the maximum
+        int i = a.vocab;
+        for (int j = row.turns - 1; j >= 0; j--) {
+            const f4v v = row.get(j);
+#pragma unroll
+            for (int e = 3; e >= 0; e--) i = v[e] == top ? row.index(j) + e : i;
+        }
+        for (int d = 32; d; d >>= 1) i = min(i, __shfl_xor(i, d));
+        if (lane == 0) atomicMin(&s.index, i);
         __syncthreads();
-        for (int d = kThreads / 2; d > 0; d >>= 1) {
-            if (t < d) part[t] += part[t + d];
+        if (t == 0) a.token[r] = s.index;
+        return;
+    }
+    const double scale = 1.4426950408889634 / (double)temp;
+    const WeightOf weight = {top, scale, min_pf > 1.0f ? 1.0 : min_pf > 0.0f ? (double)min_pf : 0.0};
+    // Logits under floor_ weigh nothing (2^-46 is 0, of 2^-44), whatever stays.
+    const double reach = (double)top - 46.0 / scale;
+    const float floor_ = reach > -(double)FLT_MAX ? (float)reach - fabsf((float)reach) * 1e-6f : -FLT_MAX;
+    // stays: logits above `last`, and the first `ties` of its `equals`
+    float last = floor_;
+    u64 ties = (u64)a.vocab, equals = 0;
+    if (top_k > 0 && top_k < a.vocab) {
+        u64 n = 0;
+        row.each([&](float x) { n += x >= floor_; });
+        n = block_scan(n, s);
+        if (t == kThreads - 1) s.before = n;
+        __syncthreads();
+        const bool fewer = (u64)top_k < s.before;            // uniform: top_k leaves out some that weigh
+        __syncthreads();
+        if (fewer) {
+            const Mark k = find_mark(row, s, floor_, top, CountOf(), [&](u64) { return (u64)top_k; });
+            last = k.value;
+            equals = k.equals;
+            ties = (u64)top_k - k.before;
+        }
+    }
+    if (!(top_p >= 1.0f)) {
+        const u64 dropped = equals > ties ? (equals - ties) * weight(last) : 0;
+        // stays: sums before it under top_p * total, so the last is where the sum reaches it
+        const Mark k = find_mark(row, s, last, top, weight, [&](u64 sum) {
+            const double lim = top_p > 0.0f ? (double)top_p * (double)(sum - dropped) : 0.0;
+            u64 need = (u64)lim;
+            if ((double)need < lim) need++;
+            return max(need, (u64)1);
+        });
+        const u64 each = weight(k.value), n = (k.need - k.before + each - 1) / each;
+        if (k.value > last) {
+            last = k.value;
+            equals = k.equals / each;
+            ties = n;
+        } else {
+            equals = k.equals / each;
+            ties = min(ties, n);
+        }
+    }
+    // more equals of the last than stay: the index of the last that does
+    int cut = a.vocab;
+    if (equals > ties) {                                     // uniform
+        u64 seen = 0;
+        for (int j = 0; j < row.turns; j++) {
+            const f4v v = row.get(j);
+            const u64 mine = (v[0] == last) + (v[1] == last) + (v[2] == last) + (v[3] == last);
+            const u64 upto = block_scan(mine, s), from = seen + upto - mine;
+            if (from < ties && ties <= from + mine) {
+                int k = (int)(ties - from);
+                for (int e = 0; e < 4; e++)
+                    if (v[e] == last && --k == 0) s.index = row.index(j) + e;
+            }
+            if (t == kThreads - 1) s.before = upto;
+            __syncthreads();
+            seen += s.before;
             __syncthreads();
         }
-        const u64 v = part[0];
-        __syncthreads();
-        return v;
-    };
-    auto mass = [&](unsigned k) -> u64 {
-        if (!k) return 0;
-        const double w = weight(row, logit_of(k));
-        return w >= min_p ? fixed(w) : 0;
-    };
-    // ties of tk beyond tn do not count: there are `ties` of them in all
-    auto count_ties = [&]() -> int {
-        u64 c = 0;
-        for (int i = t; i < V; i += kThreads) c += key_of(x[i]) == tk;
-        return (int)sum_all(c);
-    };
-    if (top_p < 1.0f || !(top_p == top_p)) {
-        const u64 wt = mass(tk);
+        cut = s.index;
+    }
+    // the draw: sums of every wave's turns, in the order of indices
+    auto turn_sum = [&](const f4v &v, int j) -> u64 {
         u64 w = 0;
-        for (int i = t; i < V; i += kThreads) {
-            const unsigned k = key_of(x[i]);
-            if (k > tk) w += mass(k);
-        }
-        const int ties = min(count_ties(), tn);
-        const u64 total = sum_all(w) + wt * ties;
-        // stays: sum before it < p * total; the last of them is where the running sum reaches ceil(p * total)
-        const double lim = top_p > 0.0f ? (double)top_p * (double)total : 0.0;
-        u64 need = (u64)lim;
-        if ((double)need < lim) need++;                     // before < lim  <=>  before < need
-        if (need < 1) need = 1;
-        unsigned key;
-        u64 before;
-        find([&](int, unsigned k) -> u64 { return mass(k); }, need - 1, &key, &before);
-        if (key > tk) {
-            tk = key;
-            tn = V;
-        }
-        if (key >= tk) {
-            const u64 w1 = mass(tk);
-            const u64 n = w1 ? (need - before + w1 - 1) / w1 : 1;
-            tn = (int)min((u64)tn, max(n, (u64)1));
-        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (v[e] > last || (v[e] == last && row.index(j) + e <= cut)) w += weight(v[e]);
+        return w;
+    };
+    for (int j = 0; j < row.turns; j++) {
+        const u64 mine = turn_sum(row.get(j), j);
+        const u64 upto = __any(mine != 0) ? wave_scan(mine) : 0;
+        if (lane == 63) s.block_sum[j * kWaves + wave] = upto;
     }
-    // the draw, in the order of indices: thread t takes a run of indices
-    const int run = (V + kThreads - 1) / kThreads, i0 = min(t * run, V), i1 = min(i0 + run, V);
-    u64 ties = 0;
-    for (int i = i0; i < i1; i++) ties += key_of(x[i]) == tk;
-    part[t] = ties;
     __syncthreads();
-    u64 seen = 0;
-    for (int j = 0; j < t; j++) seen += part[j];
+    const int blocks = row.turns * kWaves;                   // at most kThreads
+    const u64 one = t < blocks ? s.block_sum[t] : 0, upto = block_scan(one, s);
+    if (t == kThreads - 1) s.before = upto;
     __syncthreads();
-    u64 w = 0, c = seen;
-    for (int i = i0; i < i1; i++) {
-        const unsigned k = key_of(x[i]);
-        if (k > tk || (k == tk && c++ < (u64)tn)) w += mass(k);
-    }
-    part[t] = w;
+    const u64 total = s.before;
+    u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+    const u64 target = min((u64)((double)u * (double)total), total - 1);
+    if (upto - one <= target && target < upto) { s.bin = t; s.sum = upto - one; }
     __syncthreads();
-    u64 before = 0, total = 0;
-    for (int j = 0; j < kThreads; j++) {
-        if (j == t) before = total;
-        total += part[j];
-    }
-    const u64 target = (u64)((double)uf * (double)total);
-    if (before <= target && target < before + w) {
-        c = seen;
-        for (int i = i0; i < i1; i++) {
-            const unsigned k = key_of(x[i]);
-            if (k > tk || (k == tk && c++ < (u64)tn)) before += mass(k);
-            if (before > target) { a.token[blockIdx.x] = i; break; }
+    const int block = s.bin, j = block / kWaves;
+    if (wave == block % kWaves) {
+        const f4v v = row.get(j);
+        const u64 mine = turn_sum(v, j);
+        u64 c = s.sum + wave_scan(mine) - mine;
+        if (c <= target && target < c + mine) {
+            bool done = false;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (v[e] > last || (v[e] == last && row.index(j) + e <= cut)) c += weight(v[e]);
+                if (!done && c > target) { a.token[r] = row.index(j) + e; done = true; }
+            }
         }
     }
 }
@@ -206,8 +409,8 @@ using namespace ptmi;
 extern "C" int ptmi_sample_dev(const float *logits, long ld, int rows, int vocab, const float *temperature,
                                const int *top_k, const float *top_p, const float *min_p, const float *u, int *token,
                                void *stream) {
-    if (rows < 0 || vocab < 1 || vocab > (1 << 18) || ld < vocab)
-        return set_error(PTMI_ERR_ARG, "ptmi_sample: rows=%d vocab=%d (1..262144) ld=%ld", rows, vocab, ld);
+    if (rows < 0 || vocab < 1 || vocab > kMaxVocab || ld < vocab)
+        return set_error(PTMI_ERR_ARG, "ptmi_sample: rows=%d vocab=%d (1..%d) ld=%ld", rows, vocab, kMaxVocab, ld);
     if (rows == 0) return PTMI_OK;
     if (!logits || !token) return set_error(PTMI_ERR_ARG, "ptmi_sample: NULL argument");
     if ((uintptr_t)logits & 3) return set_error(PTMI_ERR_ARG, "ptmi_sample: logits not 4-byte aligned");
@@ -216,7 +419,9 @@ extern "C" int ptmi_sample_dev(const float *logits, long ld, int rows, int vocab
     DeviceScope dev;
     if ((st = dev.enter())) return st;
     const SampleArgs a = {logits, ld, vocab, temperature, top_k, top_p, min_p, u, token};
-    hipLaunchKernelGGL(k_sample_simple, dim3(rows), dim3(kThreads), 0, stream ? (hipStream_t)stream : lib_stream(), a);
+    const int n = vocab + (ld % 4 || (uintptr_t)logits & 15 ? 3 : 0);    // logits of the longest copy
+    hipLaunchKernelGGL(n <= 8192 ? k_sample<8192> : n <= 16384 ? k_sample<16384> : n <= 32768 ? k_sample<32768> : k_sample<0>,
+                       dim3(rows), dim3(kThreads), 0, stream ? (hipStream_t)stream : lib_stream(), a);
     PTMI_HIP(hipGetLastError());
     return PTMI_OK;
 }
