@@ -323,11 +323,14 @@ typedef struct {
  * numbers pool[0..*pool_count), room for n_pages of them; pages of ended
  * requests first go onto it (both in the order of requests, then of pages).
  * *pool_left gets the new count.  Rows from row_start[n_requests] on get
- * position and slot -1.  kv_len may be past, and pool_left pool_count.
- * *status = 0, or the sum of 1: pool short, 2: a request needs more than
- * table_width pages, 4: more than max_rows rows, 8: a bad length, count or
- * page number.  Then the step is refused as a whole: lengths, tables and
- * pool stay as they are and there are no rows (row_start is all 0).      */
+ * position and slot -1, and so do slots in pages that the table or the pool
+ * numbers outside [0, n_pages).  kv_len may be past, and pool_left
+ * pool_count.  *status = 0, or the sum of 1: pool short, 2: a request needs
+ * more than table_width pages, 4: more than max_rows rows, 8: a bad length or
+ * count, or more pages come back than there are.  Then the step is refused as
+ * a whole: lengths, tables and pool stay as they are and there are no rows
+ * (row_start is all 0).  At most 8192 requests, of 2^24 pages and 2^24 new
+ * tokens each.                                                           */
 int ptmi_paged_plan_dev(const int *past, const int *fresh, int n_requests, int *pool, const int *pool_count,
                         int n_pages, int page_size, int *block_table, int table_width, int *kv_len,
                         int *pool_left, int *row_start, int *row_pos, int *row_slot, int max_rows, int *status,

@@ -38,10 +38,13 @@ struct SampleArgs {
 };
 
 // ── weights ──────────────────────────────────────────────────────────────
-// 2^y for y <= 0, 0 below -46: 2^n p(f), |f| <= 1/2, p of degree 9 through
-// 2^f at the Chebyshev nodes (relative error 1.9e-14, a third of 2^-44).
+// 2^y for y in (-1000, 0]: 2^n p(f), n the nearest integer, p of degree 9
+// through 2^f at the Chebyshev nodes of [-1/2, 1/2] (relative error 1.9e-14,
+// a third of 2^-44).  y + 1.5 2^52 has n as its last bits, and n added to
+// p's exponent bits is the product.
 __device__ __forceinline__ double exp2_weight(double y) {
-    const double n = __builtin_rint(y), f = y - n;
+    constexpr double kShift = 6755399441055744.0;
+    const double n = y + kShift, f = y - (n - kShift);
     double p = 1.0205905413765595e-07;
     p = fma(p, f, 1.325964524488711e-06);
     p = fma(p, f, 1.5252672924850737e-05);
@@ -52,14 +55,16 @@ __device__ __forceinline__ double exp2_weight(double y) {
     p = fma(p, f, 0.2402265069564034);
     p = fma(p, f, 0.6931471805599462);
     p = fma(p, f, 1.0000000000000135);
-    return y < -46.0 ? 0.0 : ldexp(p, (int)n);
+    const u64 bits = (u64)__double_as_longlong(p);
+    const unsigned hi = (unsigned)(bits >> 32) + ((unsigned)__double_as_longlong(n) << 20);
+    return __longlong_as_double((long long)((u64)hi << 32 | (unsigned)bits));
 }
 // To the nearest multiple of 2^-44, as their number: w + 2^8 has them as its last bits.
 __device__ __forceinline__ u64 fixed(double w) {
     return (u64)(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0));
 }
 
-// What a search adds up: counts, or weights.
+// What a search adds up: counts, or weights (of logits at most 50/scale below the top).
 struct CountOf {
     __device__ __forceinline__ u64 operator()(float) const { return 1; }
 };
@@ -67,7 +72,7 @@ struct WeightOf {
     float top;
     double scale, min_p;             // log2(e) / temperature
     __device__ __forceinline__ u64 operator()(float x) const {
-        const double w = x == top ? 1.0 : exp2_weight(((double)x - (double)top) * scale);
+        const double w = exp2_weight(((double)x - (double)top) * scale);   // (x = top: 1 to the nearest 2^-44)
         return w >= min_p ? fixed(w) : 0;
     }
 };
@@ -127,6 +132,7 @@ __device__ __forceinline__ u64 block_scan(u64 v, SampleLds &s) {
 // they count, as 0.  LOCAL: `at` is a copy in shared memory, else the row.
 template <bool LOCAL>
 struct Row {
+    static constexpr int AHEAD = LOCAL ? 1 : 4;            // turns whose loads are on their way at once
     const f4v *at;
     int skip, vocab, turns;          // floats before the row in its first float4; float4s of a thread
     bool top_inf;
@@ -152,10 +158,15 @@ struct Row {
     }
     template <typename F>
     __device__ __forceinline__ void each(F &&f) const {    // f(logit) for all of this thread's
-        for (int j = 0; j < turns; j++) {
-            const f4v v = get(j);
+        for (int j0 = 0; j0 < turns; j0 += AHEAD) {
+            f4v v[AHEAD];
 #pragma unroll
-            for (int e = 0; e < 4; e++) f(v[e]);
+            for (int j = 0; j < AHEAD; j++) v[j] = get(min(j0 + j, turns - 1));
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++)
+                if (j0 + j < turns)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) f(v[j][e]);
         }
     }
 };
@@ -247,7 +258,7 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
 
 // CAP: logits that the copy in shared memory holds; 0: no copy.
 template <int CAP>
-__global__ __launch_bounds__(kThreads) void k_sample(SampleArgs a) {
+__global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_sample(SampleArgs a) {
     __shared__ SampleLds s;
     __shared__ f4v copy[CAP ? CAP / 4 : 1];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = blockIdx.x;
@@ -369,10 +380,18 @@ __global__ __launch_bounds__(kThreads) void k_sample(SampleArgs a) {
             if (v[e] > last || (v[e] == last && row.index(j) + e <= cut)) w += weight(v[e]);
         return w;
     };
-    for (int j = 0; j < row.turns; j++) {
-        const u64 mine = turn_sum(row.get(j), j);
-        const u64 upto = __any(mine != 0) ? wave_scan(mine) : 0;
-        if (lane == 63) s.block_sum[j * kWaves + wave] = upto;
+    constexpr int AHEAD = decltype(row)::AHEAD;
+    for (int j0 = 0; j0 < row.turns; j0 += AHEAD) {
+        f4v v[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) v[j] = row.get(min(j0 + j, row.turns - 1));
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++) {
+            if (j0 + j >= row.turns) continue;
+            const u64 mine = turn_sum(v[j], j0 + j);
+            const u64 upto = __any(mine != 0) ? wave_scan(mine) : 0;
+            if (lane == 63) s.block_sum[(j0 + j) * kWaves + wave] = upto;
+        }
     }
     __syncthreads();
     const int blocks = row.turns * kWaves;                   // at most kThreads

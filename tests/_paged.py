@@ -46,16 +46,13 @@ def plan(past, fresh, pool, n_pages, page, table, max_rows):
     rows = 0
     for i in range(S):
         p, f = int(past[i]), int(fresh[i])
-        if p < 0 or f < -1 or p + f > 2**31 - 1:
+        if p < 0 or f < -1 or p + f > 2**31 - 1 or f > 2**24 or n(p) > 2**24:
             status |= 8
             continue
         if n(p + max(f, 0)) > W:
             status |= 2
         elif f < 0:
-            ids = table[i, :n(p)].tolist()
-            if any(not 0 <= g < n_pages for g in ids):
-                status |= 8
-            give += ids
+            give += table[i, :n(p)].tolist()
         if f >= 0:
             take += n(p + f) - n(p)
             rows += f
@@ -80,7 +77,8 @@ def plan(past, fresh, pool, n_pages, page, table, max_rows):
         for j in range(n(p), n(p + f) if f >= 0 else 0):
             table[i, j] = pool.pop()
         for t in range(p, p + max(f, 0)):
-            pos[r], slot[r] = t, table[i, t // page] * page + t % page
+            pg = table[i, t // page]
+            pos[r], slot[r] = t, pg * page + t % page if 0 <= pg < n_pages else -1
             r += 1
     start[S] = r
     return kv, pool, start, pos, slot, 0

@@ -96,7 +96,7 @@ def test_plan_many_rows():
     assert check_plan(past, fresh, ids[at:].tolist(), need + 9, page, table, 45000) == 0
 
 
-@pytest.mark.parametrize("what", ["pool", "width", "rows", "past", "fresh", "overflow", "page", "poolpage", "count", "back"])
+@pytest.mark.parametrize("what", ["pool", "width", "rows", "past", "fresh", "overflow", "huge", "count", "back"])
 def test_plan_refuses_as_a_whole(what):
     past, fresh, page, n_pages = [20, 3, 16], [5, -1, 20], 8, 20
     table = np.full((3, 6), -1, np.int32)
@@ -115,10 +115,9 @@ def test_plan_refuses_as_a_whole(what):
         fresh[0] = -2
     elif what == "overflow":
         past[0], fresh[0] = 2**31 - 2, 9
-    elif what == "page":
-        table[1, 0] = 20
-    elif what == "poolpage":
-        pool[3] = -4
+    elif what == "huge":                                     # sums past 32 bits
+        fresh[:] = [2**31 - 100, 2**31 - 100, 2**31 - 100]
+        past[:] = [0, 0, 0]
     elif what == "count":
         pool = list(range(20)) + [3]
     elif what == "back":                                     # more pages come back than there is room for
@@ -127,12 +126,23 @@ def test_plan_refuses_as_a_whole(what):
         g = run_plan(past, fresh, pool[:20], n_pages, page, table, max_rows)
         assert g["status"][0] == 8
         return
-    if what == "poolpage":                                   # the restatement hands out what the pool holds
-        g = run_plan(past, fresh, pool, n_pages, page, table, max_rows)
-        assert g["status"][0] == 8 and g["start"][:4].tolist() == [0] * 4 and np.array_equal(g["table"], table)
-        assert g["slot"][:max_rows].tolist() == [-1] * max_rows and g["left"][0] == 4
-        return
     assert check_plan(past, fresh, pool, n_pages, page, table, max_rows) != 0
+
+
+def test_plan_passes_on_bad_page_numbers():
+    """Numbers outside the cache move as they are, and their positions have no slot."""
+    table = np.full((3, 4), -1, np.int32)
+    table[0, :3], table[1, :1], table[2, :2] = (7, 2**31 - 1, 9), (-5,), (20, 1)
+    # the last request needs five pages of a table of four: refused for that, not for the numbers
+    assert check_plan([17, 8, 16], [9, -1, 20], [11, 2**30, 13, -2**31], 20, 8, table, 40) == 2
+    assert check_plan([17, 8, 16], [9, -1, 16], [11, 2**30, 13, -2**31], 20, 8, table, 40) == 0
+
+
+def test_plan_of_most_requests():
+    rng = np.random.default_rng(3)
+    for S in (8192, 8191):
+        past, fresh, pool, n_pages, table, rows = make_requests(rng, S, 16, 20, 2, 0.2)
+        assert check_plan(past, fresh, pool, n_pages, 16, table, rows, alias=S == 8191) == 0
 
 
 def test_plan_without_requests():

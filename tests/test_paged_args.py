@@ -73,7 +73,7 @@ def test_attention_refuses(bad):
     assert attend(cache(), **bad) == ARG
 
 
-@pytest.mark.parametrize("bad", [dict(n=-1), dict(max_rows=-1), dict(n_pages=0), dict(page=0), dict(width=0),
+@pytest.mark.parametrize("bad", [dict(n=-1), dict(n=8193), dict(max_rows=-1), dict(n_pages=0), dict(page=0), dict(width=0),
                                  dict(n_pages=1 << 16, page=1 << 15), dict(pool=None), dict(count=None), dict(left=None),
                                  dict(start=None), dict(status=None), dict(past=None), dict(fresh=None), dict(table=None),
                                  dict(kv=None), dict(pos=None), dict(slot=None)], ids=str)
