@@ -392,6 +392,37 @@ size_t ptmi_paged_attention_work(const ptmi_pages_t *pages, int n_heads, int max
 int ptmi_sample_dev(const float *logits, long ld, int rows, int vocab, const float *temperature, const int *top_k,
                     const float *top_p, const float *min_p, const float *u, int *token, void *stream);
 
+/* ── many requests through a model ────────────────────────────────────
+ * max_requests requests at a time, each with its place 0..max_requests-1,
+ * over one paged cache of n_pages pages of page_size positions in every
+ * layer (cache_type PTMI_F32 or PTMI_BF16), at most max_rows new tokens a
+ * step.  It holds the weights of m's blob, not m itself.  Continuous
+ * batching of pt_generate's loop (pitorch/text/pt_text.c:314-361): prompts
+ * (whole or in pieces) and single tokens share a step, requests come and go.
+ * At most 2^20 rows a step and 8192 requests.                           */
+typedef struct ptmi_batch ptmi_batch_t;
+/* Host arrays by request, as ptmi_sample_dev takes them by row; NULL = off,
+ * without temperature the choice is greedy.                             */
+typedef struct {
+    const float *temperature;
+    const int   *top_k;
+    const float *top_p, *min_p, *u;
+} ptmi_sampling_t;
+int  ptmi_batch_create(ptmi_model_t *m, int max_requests, int max_rows, int n_pages, int page_size, int cache_type,
+                       ptmi_batch_t **out);
+void ptmi_batch_destroy(ptmi_batch_t *b);
+/* One step: request i takes n_new[i] tokens (0: it sits out; -1: it has
+ * ended, its pages are free and its place empty), given in `tokens` request
+ * by request.  next[i] = the token chosen after the last of them, -1 where
+ * there are none (next may be NULL).  A step that does not fit (positions
+ * past seq_len, more rows than max_rows, too few free pages) is refused with
+ * PTMI_ERR_STATE and changes nothing.                                   */
+int  ptmi_batch_step(ptmi_batch_t *b, const int *n_new, const int *tokens, const ptmi_sampling_t *sampling, int *next);
+/* The last step's logits [vocab] of a request that had tokens in it. */
+int  ptmi_batch_logits(ptmi_batch_t *b, int request, float *out);
+int  ptmi_batch_length(const ptmi_batch_t *b, int request);    /* positions of a request */
+int  ptmi_batch_free_pages(const ptmi_batch_t *b);
+
 #ifdef __cplusplus
 }
 #endif

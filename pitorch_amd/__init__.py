@@ -11,6 +11,7 @@ is no CPU fallback: if the libraries are missing, loading raises.
 from ._ffi import (  # noqa: F401
     BF16,
     F32,
+    Batch,
     Model,
     Pages,
     PtmiError,

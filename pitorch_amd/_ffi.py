@@ -26,6 +26,11 @@ class Pages(ctypes.Structure):
 F32, BF16 = 0, 1    # ptmi_pages_t.type
 
 
+class Sampling(ctypes.Structure):
+    """ptmi_sampling_t (include/ptmi.h)."""
+    _fields_ = [("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp), ("u", _vp)]
+
+
 def lib_dir():
     return os.path.join(_HERE, "lib")
 
@@ -108,6 +113,12 @@ def load_ptmi():
     _sig(L, "ptmi_paged_attention_dev", i, [pages, _vp, i, _vp, _vp, i, i, _vp, lg, _vp, lg, i, i, f, _vp, sz, _vp])
     _sig(L, "ptmi_paged_attention_work", sz, [pages, i, i])
     _sig(L, "ptmi_sample_dev", i, [_vp, lg, i, i, _vp, _vp, _vp, _vp, _vp, _vp, _vp])
+    _sig(L, "ptmi_batch_create", i, [_vp, i, i, i, i, i, ctypes.POINTER(_vp)])
+    _sig(L, "ptmi_batch_destroy", None, [_vp])
+    _sig(L, "ptmi_batch_step", i, [_vp, _vp, _vp, ctypes.POINTER(Sampling), _vp])
+    _sig(L, "ptmi_batch_logits", i, [_vp, i, _vp])
+    _sig(L, "ptmi_batch_length", i, [_vp, i])
+    _sig(L, "ptmi_batch_free_pages", i, [_vp])
     _ptmi = L
     return L
 
@@ -338,3 +349,54 @@ class Model:
         out = np.empty(n, dtype=np.float32)
         check(self.L.ptmi_model_read_grads(self.h, out.ctypes.data_as(_c_float_p), n))
         return out
+
+
+class Batch:
+    """Many requests through one model over a paged cache (ptmi_batch_*)."""
+
+    def __init__(self, model, max_requests, max_rows, n_pages, page_size=16, cache_type=F32):
+        self.L = load_ptmi()
+        self.blob = model.blob             # held: the weights' registration goes by its address
+        self.max_requests, self.vocab = max_requests, model.vocab
+        h = _vp()
+        check(self.L.ptmi_batch_create(model.h, max_requests, max_rows, n_pages, page_size, cache_type, ctypes.byref(h)))
+        self.h = h
+
+    def close(self):
+        if self.h:
+            self.L.ptmi_batch_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def step(self, new, temperature=None, top_k=None, top_p=None, min_p=None, u=None):
+        """new: {request: its tokens, or None: it has ended}; the parameters by request (max_requests values).
+        Returns {request: next token} of those with tokens."""
+        n_new, tokens = np.zeros(self.max_requests, np.int32), []
+        for r in sorted(new):
+            n_new[r] = -1 if new[r] is None else len(new[r])
+            tokens += [] if new[r] is None else list(new[r])
+        tokens = np.array(tokens, np.int32)
+        kept = [None if a is None else np.ascontiguousarray(a, t) for a, t in
+                ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32), (u, np.float32))]
+        if any(a is not None and a.size != self.max_requests for a in kept):
+            raise ValueError("sampling parameters: one value per request")
+        s = Sampling(*[None if a is None else a.ctypes.data for a in kept])
+        out = np.empty(self.max_requests, np.int32)
+        check(self.L.ptmi_batch_step(self.h, _ptr(n_new), _ptr(tokens), ctypes.byref(s), _ptr(out)))
+        return {int(r): int(out[r]) for r in np.flatnonzero(n_new > 0)}
+
+    def logits(self, request):
+        out = np.empty(self.vocab, np.float32)
+        check(self.L.ptmi_batch_logits(self.h, int(request), _ptr(out)))
+        return out
+
+    def length(self, request):
+        return self.L.ptmi_batch_length(self.h, int(request))
+
+    def free_pages(self):
+        return self.L.ptmi_batch_free_pages(self.h)
