@@ -195,6 +195,12 @@ struct Split {
     }
 };
 
+// Lane i's value, i the same in all lanes.
+__device__ __forceinline__ long lane_value(long v, int i) {
+    return (long)((unsigned long)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 |
+                  (unsigned)__builtin_amdgcn_readlane((int)v, i));
+}
+
 // One item of the axis: a head's keys for one tile of rows, units [a, b).
 struct Item {
     int s, kvh, tile;
@@ -214,15 +220,15 @@ __device__ Item axis_item(const AttnArgs &a, Axis &x, long u) {
     if constexpr (TILE) {                                  // lane i: tile 64 k + i
         const int tt = a.tile_tokens, lane = threadIdx.x & 63;
         const long mine = (tile_keys0(a, it.r) + (unsigned)(lane * tt)) / kUnit, upto = wave_scan(mine);
-        const long s = __shfl(upto, 63);
+        const long s = lane_value(upto, 63);
         long k = 0, w = u - it.a;
         while (blocks_before(k + 1, s, tt) <= w) k++;
         w -= blocks_before(k, s, tt);
         const long end = upto + (long)(lane + 1) * tt * k;
         const int i = __popcll(__ballot(end <= w));         // (under 64: w lies in block k)
         it.tile = (int)(64 * k) + i;
-        it.b = it.a + blocks_before(k, s, tt) + __shfl(end, i);
-        it.a = it.b - __shfl(mine, i) - tt * k;
+        it.b = it.a + blocks_before(k, s, tt) + lane_value(end, i);
+        it.a = it.b - lane_value(mine, i) - tt * k;
     }
     return it;
 }
@@ -875,41 +881,22 @@ __global__ __launch_bounds__(64 * tile_waves(DT), 2) void k_attn_tile(AttnArgs a
         auto page_at = [&](int b) { return b < b1 ? page_of(a, it.s, b * kUnit + lane, end) : -1; };
         const int turn = (wave - b0) & (NW - 1);             // this wave's first unit, from b0
         int pg = page_at(b0 + turn);
+        // q: columns 16 ks + 8 half .. of the row (on its way while the page numbers are)
+        f4v qx[KS][2];
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int d = 16 * ks + 8 * half + 4 * j;
+                qx[ks][j] = f4v{0.f, 0.f, 0.f, 0.f};
+                if (live && (!PAD || d < hd)) qx[ks][j] = *reinterpret_cast<const f4v *>(a.q + row * a.ldq + head * hd + d);
+            }
         __syncthreads();                                     // the last item's readers are done
         if (turn < 3) {
             put_off(b0 + turn, pg);
             pg = page_at(b0 + turn + NW);
         }
         if (tid < 4) lds.odd[tid] = 0;
-        // q: columns 16 ks + 8 half .. of the row, scaled, split
-        h8v qh[KS], ql[KS];
-        int qe;
-        {
-            f4v x[KS][2];
-            unsigned top = 0;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int d = 16 * ks + 8 * half + 4 * j;
-                    x[ks][j] = f4v{0.f, 0.f, 0.f, 0.f};
-                    if (live && (!PAD || d < hd))
-                        x[ks][j] = *reinterpret_cast<const f4v *>(a.q + row * a.ldq + head * hd + d) * a.qscale;
-                    top = finite_top(top, x[ks][j]);
-                }
-            const LanePair pr = pl32(__uint_as_float(top));
-            qe = max((int)(__float_as_uint(fmaxf(pr.lo, pr.hi)) >> 23) - 127, -100) - kTop;
-            const float sc = pow2(-qe);
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    h4v h, r;
-                    split4(x[ks][j] * sc, m1, h, r);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) { qh[ks][4 * j + e] = h[e]; ql[ks][4 * j + e] = r[e]; }
-                }
-        }
         __syncthreads();
         // a unit's keys and values as they come: K thread (key, i): float4s i, i + KL, ..; V task (quad, c):
         // keys 4 quad.., float4 c
@@ -1023,11 +1010,37 @@ __global__ __launch_bounds__(64 * tile_waves(DT), 2) void k_attn_tile(AttnArgs a
             for (int r = 0; r < 16; r++) acc[d][r] = 0.0f;
         float m = -INFINITY, l = 0.0f;
         int acc_e = -1000;                                   // acc counts in 2^acc_e
+        RawK rk0;
+        RawV rv0;
         if (b0 < b1) {                                       // unit b0 to LDS, b0 + 1 to registers
-            RawK rk0;
-            RawV rv0;
             load(b0, rk0, rv0);
             load(b0 + 1, rk, rv);
+        }
+        h8v qh[KS], ql[KS];
+        int qe;
+        {
+            unsigned top = 0;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    qx[ks][j] *= a.qscale;
+                    top = finite_top(top, qx[ks][j]);
+                }
+            const LanePair pr = pl32(__uint_as_float(top));
+            qe = max((int)(__float_as_uint(fmaxf(pr.lo, pr.hi)) >> 23) - 127, -100) - kTop;
+            const float sc = pow2(-qe);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    h4v h, r;
+                    split4(qx[ks][j] * sc, m1, h, r);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { qh[ks][4 * j + e] = h[e]; ql[ks][4 * j + e] = r[e]; }
+                }
+        }
+        if (b0 < b1) {
             tops(b0, rk0, rv0);
             tops(b0 + 1, rk, rv);
             __syncthreads();
@@ -1252,16 +1265,43 @@ __global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, int n_few, c
     if (c.parts == 0) return;
     auto part_of = [&](int p) { return tile_parts + (long)(2 * (w + p) + (p == 0)) * tile_part(DT); };
     const int tt = a.tile_tokens, t0 = c.tile * tt;
-    for (int e = tid; e < 64 * NW * DT; e += kThreads) {     // as the lanes of the tile's waves
-        const int lane = e & 63, wave = (e >> 6) % NW, q = 4 * (e / (64 * NW)) + q0;
-        const int mrow = wave * 32 + (lane & 31), at = 8 * q + 4 * (lane >> 5);
+    constexpr int NE = 64 * NW * DT / kThreads;              // float4s of a thread
+    Join j[NE];
+    float *to[NE];
+    long ml[NE], at[NE];
+#pragma unroll
+    for (int i = 0; i < NE; i++) {                           // as the lanes of the tile's waves
+        const int e = tid + i * kThreads, lane = e & 63, wave = (e >> 6) % NW, q = 4 * (e / (64 * NW)) + q0;
+        const int mrow = wave * 32 + (lane & 31), col = 8 * q + 4 * (lane >> 5);
         const int tok = t0 + a.group.quot(mrow), row = c.row0 + tok;
-        if (!(mrow < tt * G && tok < c.n && (unsigned)row < (unsigned)a.rows && at < hd)) continue;
-        Join j = {-INFINITY, 0.0f, {0.f, 0.f, 0.f, 0.f}};
-        join_parts<2>(j, 0, 1, c.parts, 32 * NW * 32 * DT + 2 * mrow, 4l * ((wave * 4 * DT + q) * 64 + lane), part_of);
-        *reinterpret_cast<f4v *>(a.out + row * a.ldo + (c.kvh * G + mrow - (tok - t0) * G) * (long)hd + at) =
-            j.o * (j.l == 0.0f ? 0.0f : 1.0f / j.l);
+        const bool live = mrow < tt * G && tok < c.n && (unsigned)row < (unsigned)a.rows && col < hd;
+        to[i] = live ? a.out + row * a.ldo + (c.kvh * G + mrow - (tok - t0) * G) * (long)hd + col : nullptr;
+        ml[i] = 32 * NW * 32 * DT + 2 * mrow;
+        at[i] = 4l * ((wave * 4 * DT + q) * 64 + lane);
+        j[i] = Join{-INFINITY, 0.0f, {0.f, 0.f, 0.f, 0.f}};
     }
+    for (int p0 = 0; p0 < c.parts; p0 += 2) {
+        const float *p[2] = {part_of(p0), part_of(min(p0 + 1, c.parts - 1))};
+        f2v pml[2][NE];
+        f4v po[2][NE];
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < NE; i++) {
+                if (!to[i]) continue;
+                pml[s][i] = *reinterpret_cast<const f2v *>(p[s] + ml[i]);
+                po[s][i] = *reinterpret_cast<const f4v *>(p[s] + at[i]);
+            }
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+            if (p0 + s < c.parts)
+#pragma unroll
+                for (int i = 0; i < NE; i++)
+                    if (to[i]) j[i].add(pml[s][i].x, pml[s][i].y, po[s][i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NE; i++)
+        if (to[i]) *reinterpret_cast<f4v *>(to[i]) = j[i].o * (j[i].l == 0.0f ? 0.0f : 1.0f / j[i].l);
 }
 
 // ── launch ───────────────────────────────────────────────────────────────
