@@ -17,8 +17,10 @@
 // (m, l, o) in the workspace, and k_attn_join adds such parts up in order.
 #include "ptmi_paged.h"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
+#include <unordered_map>
 
 namespace ptmi {
 
@@ -342,7 +344,7 @@ __device__ __forceinline__ void few_load(const AttnArgs &a, FewBlock<HQ, PAD, BF
 }
 
 template <int HQ, bool PAD, bool BF16>
-__global__ __launch_bounds__(kThreads) void k_attn_few(AttnArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void k_attn_few(AttnArgs a) {
     constexpr int C4 = HQ > 4 ? 2 : 1, NC = 4 * C4, FP = few_pitch(HQ / 2), PITCH = FP + 4, NW = kThreads / 64;
     __shared__ Axis axis;
     __shared__ __align__(16) float red[NW * kFewRows * PITCH];
@@ -1305,7 +1307,11 @@ __global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, int n_few, c
 }
 
 // ── launch ───────────────────────────────────────────────────────────────
-constexpr int kFewGroups = 1024;                            // workgroups: what the chip holds at once
+// Workgroups: what the chip holds at once.  More would split heads further
+// and start anew (64 requests of 32 heads on 4, 1024 bf16 positions of 128:
+// 104 us on 1024 workgroups, 54 on the 512 that fit), fewer leave it idle
+// (1024 requests of 12 heads, 100 positions of 64: 168 us on 512, 133 on 1024).
+constexpr int kFewGroups = 1024;                            // the most for few rows
 constexpr int kTileGroups = 512;
 constexpr int tile_groups(int dt) { return 2048 / tile_waves(dt); }
 
@@ -1336,6 +1342,17 @@ template <int DT>
 Fn tile_fn(int hd, bool b16) {
     return hd == 32 * DT ? (b16 ? k_attn_tile<DT, false, true> : k_attn_tile<DT, false, false>)
                          : (b16 ? k_attn_tile<DT, true, true> : k_attn_tile<DT, true, false>);
+}
+
+int few_groups(Fn fn) {
+    static std::unordered_map<Fn, int> known;
+    int &n = known[fn];
+    if (n == 0) {
+        int per_cu = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, (const void *)fn, kThreads, 0) != hipSuccess) per_cu = 2;
+        n = std::min(kFewGroups, 256 * std::max(1, per_cu));
+    }
+    return n;
 }
 
 // Which kernels a call runs.
@@ -1387,7 +1404,7 @@ int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, 
     int st = check_heads("ptmi_paged_attention", pages, n_heads, max_new);
     if (st) return st;
     const ptmi_pages_t &p = *pages;
-    if (n_requests < 0 || table_width < 1 || rows < 0 || !std::isfinite(scale))
+    if (n_requests < 0 || table_width < 1 || rows < 0 || !std::isfinite(scale * 1.44269504f))
         return set_error(PTMI_ERR_ARG, "ptmi_paged_attention: n_requests=%d table_width=%d rows=%d scale=%g", n_requests,
                          table_width, rows, (double)scale);
     if ((long long)table_width * p.page_size > INT_MAX - 4096)
@@ -1417,10 +1434,12 @@ int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, 
     const bool b16 = p.type == PTMI_BF16;
     const int hd = p.head_dim;
     const int dt = tile_dt(hd), n_tile = plan.tile ? tile_groups(dt) : 1;
+    int n_few = 1;
     if (plan.few) {
         const Fn fn = plan.stream ? stream_fn(plan.stream, p) : dt == 1 ? few_fn<2>(hd, b16) : dt == 2 ? few_fn<4>(hd, b16) : dt == 3 ? few_fn<6>(hd, b16)
                     : few_fn<8>(hd, b16);
-        hipLaunchKernelGGL(fn, dim3(kFewGroups), dim3(kThreads), 0, s, a);
+        n_few = few_groups(fn);
+        hipLaunchKernelGGL(fn, dim3(n_few), dim3(kThreads), 0, s, a);
     }
     if (plan.tile) {
         const Fn fn = dt == 1 ? tile_fn<1>(hd, b16) : dt == 2 ? tile_fn<2>(hd, b16) : dt == 3 ? tile_fn<3>(hd, b16)
@@ -1433,9 +1452,9 @@ int ptmi_paged_attention_dev(const ptmi_pages_t *pages, const int *block_table, 
     // One unit a head and nothing but single rows: nothing is ever cut.
     if (plan.tile || (long)table_width * p.page_size > kUnit) {
         // (the last workgroup's stretch ends with an item)
-        const int n_few = plan.few ? kFewGroups - 1 : 0, n_join = plan.tile ? 4 * (n_tile - 1) : 0;
+        const int n_join = 4 * (n_tile - 1);
         const JoinFn join = dt == 1 ? k_attn_join<1> : dt == 2 ? k_attn_join<2> : dt == 3 ? k_attn_join<3> : k_attn_join<4>;
-        hipLaunchKernelGGL(join, dim3(n_few + n_join), dim3(kThreads), 0, s, a, n_few, a.cuts + kFewGroups,
+        hipLaunchKernelGGL(join, dim3(n_few - 1 + n_join), dim3(kThreads), 0, s, a, n_few - 1, a.cuts + kFewGroups,
                            (const float *)work + plan.tile_at);
     }
     PTMI_HIP(hipGetLastError());

@@ -64,7 +64,7 @@ __device__ __forceinline__ u64 fixed(double w) {
     return (u64)(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0));
 }
 
-// What a search adds up: counts, or weights (of logits at most 50/scale below the top).
+// What a search adds up: counts, or weights.
 struct CountOf {
     __device__ __forceinline__ u64 operator()(float) const { return 1; }
 };
@@ -72,7 +72,7 @@ struct WeightOf {
     float top;
     double scale, min_p;             // log2(e) / temperature
     __device__ __forceinline__ u64 operator()(float x) const {
-        const double w = exp2_weight(((double)x - (double)top) * scale);   // (x = top: 1 to the nearest 2^-44)
+        const double w = exp2_weight(fmax(((double)x - (double)top) * scale, -60.0));   // (x = top: 1 to the nearest 2^-44)
         return w >= min_p ? fixed(w) : 0;
     }
 };

@@ -326,6 +326,9 @@ CASES = [
     ([(60, 50)], 3, 3, 100, 16, pa.F32, "tokens"),
     ([(60, 33)], 20, 1, 64, 16, pa.F32, "tokens"),
     ([(1000, 128)], 1, 1, 96, 32, pa.F32, "tokens"),
+    ([(0, 300), (513, 257)], 1, 1, 128, 16, pa.F32, "tokens"),
+    ([(5, 9000)], 1, 1, 4, 64, pa.F32, "tokens"),                  # more than 64 tiles of rows
+    ([(100, 3), (7, 64)], 128, 1, 4, 16, pa.F32, "tokens"),        # the most heads that share one
 ]
 
 
@@ -407,6 +410,43 @@ def test_attention_of_values_that_are_not_finite(new, what, bad):
         assert np.isnan(got[new:, 1][q_sign[new:] > 0 if bad == np.inf else slice(None)]).all()
     else:
         assert not np.isfinite(got[new:, 1, 5]).any() and np.isfinite(np.delete(got[new:, 1], 5, 1)).all()
+
+
+@pytest.mark.parametrize("new", [2, 3, 8, 70])
+@pytest.mark.parametrize("kind", [pa.F32, pa.BF16])
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_attention_of_new_tokens_that_are_not_finite(new, kind, what, bad):
+    """A new token's key or value reaches the rows from its own on, none before it."""
+    at = 2 * new // 3                                         # the new token
+    reqs = [(37, new), (20, new)]
+    base, _, _ = run_attention(reqs, 2, 2, 64, 16, kind, seed=8)
+    q = np.zeros(2 * new)
+
+    def edit(d):
+        q[:] = d["q"][:, 1, 5]
+        pos = 37 + at
+        d[what][d["table"][0, pos // 16] * 16 + pos % 16, 1, 5] = bad
+    got, _, _ = run_attention(reqs, 2, 2, 64, 16, kind, seed=8, edit=edit)
+    # (the scale of the tile's keys may have moved with them: a rounding, not the bits)
+    assert np.isfinite(got[:at]).all() and np.allclose(got[:at], base[:at], rtol=0, atol=2e-5)
+    assert np.allclose(got[:, 0], base[:, 0], rtol=0, atol=2e-5) and np.allclose(got[new:], base[new:], rtol=0, atol=2e-5)
+    if what == "v":
+        assert not np.isfinite(got[at:new, 1, 5]).any()
+        rest = [i for i in range(64) if i != 5]
+        assert np.allclose(got[at:new, 1][:, rest], base[at:new, 1][:, rest], rtol=0, atol=2e-5)
+    else:
+        seen = q[at:new] > 0 if bad == np.inf else slice(None)
+        assert np.isnan(got[at:new, 1][seen]).all()
+
+
+@pytest.mark.parametrize("news", [(0, 1), (0, 1, 2), (1, 3, 9), (0, 1, 25)])
+def test_attention_of_many_requests(news):
+    """More requests than a workgroup looks at in one turn."""
+    rng = np.random.default_rng(len(news) + news[-1])
+    reqs = [(int(rng.integers(0, 40)), int(rng.choice(news))) for _ in range(600)]
+    assert_close(*run_attention(reqs, 2, 1, 32, 8, pa.F32, seed=12))
+    assert_close(*run_attention(reqs, 1, 1, 16, 8, pa.BF16, seed=13, max_new=0))
 
 
 @pytest.mark.parametrize("new", [1, 2, 40])

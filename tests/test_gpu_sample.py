@@ -107,6 +107,18 @@ def test_parameters_out_of_range():
             u=[.5, .5, -1, 2, .3, .3, .3, .3, .3, nan, .7, .7])
 
 
+def test_temperatures_that_choose():
+    """Logits nearer to the maximum than a millionth of it, at temperatures that tell them apart all the same."""
+    x = np.full((8, 300), -5.0, np.float32)
+    x[:, 40:60] = np.float32(1000) + np.arange(20, dtype=np.float32) * np.float32(2.0**-14)
+    x[:, 47] = x[:, 59]                                       # two maxima
+    for t in (1e-38, 1e-30, 1e-9, 1e-5):
+        got = compare(x, temperature=[t] * 8, u=np.linspace(0, 0.99, 8))
+        if t < 1e-6:
+            assert got.tolist() == [47] * 4 + [59] * 4
+    compare(x, temperature=[1e30, 3e38] * 4, u=np.linspace(0, 0.99, 8))
+
+
 @pytest.mark.parametrize("V", [1000, 32000])
 def test_equal_logits(V):
     """Whole weights: every border is met exactly, and the first of equals counts."""

@@ -65,7 +65,7 @@ def test_store_refuses(bad):
 
 
 @pytest.mark.parametrize("bad", [dict(n=-1), dict(width=0), dict(rows=-1), dict(new=-1), dict(heads=0), dict(heads=3),
-                                 dict(scale=float("nan")), dict(scale=float("inf")), dict(table=None), dict(start=None),
+                                 dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(table=None), dict(start=None),
                                  dict(kv=None), dict(q=None), dict(out=None), dict(work=None), dict(q=P + 4), dict(out=P),
                                  dict(ldq=252), dict(ldo=257), dict(work=P + 8), dict(work_bytes=0),
                                  dict(width=1 << 27)], ids=str)
