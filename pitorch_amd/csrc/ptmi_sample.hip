@@ -38,23 +38,29 @@ struct SampleArgs {
 };
 
 // ── weights ──────────────────────────────────────────────────────────────
+// The coefficients of exp2_weight's polynomial, in scalar registers (as
+// literals each would first be copied into a vector register for its fma:
+// half as many instructions again).
+struct Exp2Poly {
+    double c[10];
+    __device__ __forceinline__ Exp2Poly()
+        : c{1.0000000000000135, 0.6931471805599462, 0.2402265069564034, 0.05550410866465167, 0.009618129193934313,
+            0.0013333558200794592, 0.0001540343375125101, 1.5252672924850737e-05, 1.325964524488711e-06,
+            1.0205905413765595e-07} {
+#pragma unroll
+        for (int i = 0; i < 10; i++) asm("" : "+s"(c[i]));
+    }
+};
 // 2^y for y in (-1000, 0]: 2^n p(f), n the nearest integer, p of degree 9
 // through 2^f at the Chebyshev nodes of [-1/2, 1/2] (relative error 1.9e-14,
 // a third of 2^-44).  y + 1.5 2^52 has n as its last bits, and n added to
 // p's exponent bits is the product.
-__device__ __forceinline__ double exp2_weight(double y) {
+__device__ __forceinline__ double exp2_weight(const Exp2Poly &q, double y) {
     constexpr double kShift = 6755399441055744.0;
     const double n = y + kShift, f = y - (n - kShift);
-    double p = 1.0205905413765595e-07;
-    p = fma(p, f, 1.325964524488711e-06);
-    p = fma(p, f, 1.5252672924850737e-05);
-    p = fma(p, f, 0.0001540343375125101);
-    p = fma(p, f, 0.0013333558200794592);
-    p = fma(p, f, 0.009618129193934313);
-    p = fma(p, f, 0.05550410866465167);
-    p = fma(p, f, 0.2402265069564034);
-    p = fma(p, f, 0.6931471805599462);
-    p = fma(p, f, 1.0000000000000135);
+    double p = q.c[9];
+#pragma unroll
+    for (int i = 8; i >= 0; i--) p = fma(p, f, q.c[i]);
     const u64 bits = (u64)__double_as_longlong(p);
     const unsigned hi = (unsigned)(bits >> 32) + ((unsigned)__double_as_longlong(n) << 20);
     return __longlong_as_double((long long)((u64)hi << 32 | (unsigned)bits));
@@ -69,10 +75,11 @@ struct CountOf {
     __device__ __forceinline__ u64 operator()(float) const { return 1; }
 };
 struct WeightOf {
+    Exp2Poly poly;
     float top;
     double scale, min_p;             // log2(e) / temperature
     __device__ __forceinline__ u64 operator()(float x) const {
-        const double w = exp2_weight(fmax(((double)x - (double)top) * scale, -60.0));   // (x = top: 1 to the nearest 2^-44)
+        const double w = exp2_weight(poly, fmax(((double)x - (double)top) * scale, -60.0));   // (x = top: 1 to the nearest 2^-44)
         return w >= min_p ? fixed(w) : 0;
     }
 };
@@ -156,17 +163,16 @@ struct Row {
             for (int e = 0; e < 4; e++) v[e] = v[e] == INFINITY ? 0.0f : -INFINITY;
         return v;
     }
+    // f(four logits) for all of this thread's: four at a time, because a weight is a chain of dependent operations
     template <typename F>
-    __device__ __forceinline__ void each(F &&f) const {    // f(logit) for all of this thread's
+    __device__ __forceinline__ void each(F &&f) const {
         for (int j0 = 0; j0 < turns; j0 += AHEAD) {
             f4v v[AHEAD];
 #pragma unroll
             for (int j = 0; j < AHEAD; j++) v[j] = get(min(j0 + j, turns - 1));
 #pragma unroll
             for (int j = 0; j < AHEAD; j++)
-                if (j0 + j < turns)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) f(v[j][e]);
+                if (j0 + j < turns) f(v[j]);
         }
     }
 };
@@ -182,17 +188,25 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
     Mark k = {hi, 0, 0, 0};
     bool first = true;
     for (;;) {
-        // lo < hi fall into different bins (but where they are equal), so the bounds close in
-        const double top = hi, inv = lo < hi ? kBins / (top - (double)lo) : 0.0;
-        auto bin_of = [&](float x) { return min((int)((top - (double)x) * inv), kBins - 1); };
+        // Bins of (hi - x)/2, which no pair of floats overflows.  lo < hi fall into different ones, so the bounds
+        // close in; where even half their distance is nothing (subnormals next to each other), hi alone is a bin.
+        const float half = 0.5f * hi, range = half - 0.5f * lo;
+        const bool apart = range > 0.0f;
+        const float pre = range < 1e-20f ? 0x1p100f : 1.0f, inv = apart ? (float)kBins / (range * pre) : 0.0f;   // (finite)
+        auto bin_of = [&](float x) {
+            const int b = min((int)(fmaf(-0.5f, x, half) * pre * inv), kBins - 1);
+            return apart || x == hi ? b : 1;
+        };
         s.bins[t] = s.bins[t + kThreads] = 0;
         if (t == 0) { s.members = 0; s.lo = 0xFFFFFFFFu; s.hi = 0; }
         __syncthreads();
-        row.each([&](float x) {
-            if (x >= lo && x <= hi) {
-                const u64 w = measure(x);
-                if (w) atomicAdd(&s.bins[bin_of(x)], w);
-            }
+        row.each([&](const f4v &x) {
+            u64 w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = measure(x[e]);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (x[e] >= lo && x[e] <= hi && w[e]) atomicAdd(&s.bins[bin_of(x[e])], w[e]);
         });
         __syncthreads();
         const u64 b0 = s.bins[2 * t], b1 = s.bins[2 * t + 1], c1 = block_scan(b0 + b1, s), c0 = c1 - b1, cb = c0 - b0;
@@ -212,14 +226,20 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
         k.value = hi;
         if (!(lo < hi)) { __syncthreads(); return k; }      // all equal
         float least = INFINITY, most = -INFINITY;
-        row.each([&](float x) {
-            if (x >= lo && x <= hi && bin_of(x) == bin) {
-                least = fminf(least, x);
-                most = fmaxf(most, x);
+        row.each([&](const f4v &x) {
+            unsigned in = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) in |= x[e] >= lo && x[e] <= hi && bin_of(x[e]) == bin ? 1u << e : 0;
+            if (!in) return;
+            for (int e = 0; e < 4; e++) {
+                if (!(in >> e & 1)) continue;
+                const float y = e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3];
+                least = fminf(least, y);
+                most = fmaxf(most, y);
                 // (the count stops a little above kList)
                 if (*(volatile int *)&s.members <= kList) {
                     const int at = atomicAdd(&s.members, 1);
-                    if (at < kList) { s.list_x[at] = x; s.list_w[at] = measure(x); }
+                    if (at < kList) { s.list_x[at] = y; s.list_w[at] = measure(y); }
                 }
             }
         });
@@ -311,7 +331,7 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
         return;
     }
     const double scale = 1.4426950408889634 / (double)temp;
-    const WeightOf weight = {top, scale, min_pf > 1.0f ? 1.0 : min_pf > 0.0f ? (double)min_pf : 0.0};
+    const WeightOf weight = {Exp2Poly(), top, scale, min_pf > 1.0f ? 1.0 : min_pf > 0.0f ? (double)min_pf : 0.0};
     // Logits under floor_ weigh nothing (2^-46 is 0, of 2^-44), whatever stays.
     const double reach = (double)top - 46.0 / scale;
     const float floor_ = reach > -(double)FLT_MAX ? (float)reach - fabsf((float)reach) * 1e-6f : -FLT_MAX;
@@ -320,7 +340,7 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     u64 ties = (u64)a.vocab, equals = 0;
     if (top_k > 0 && top_k < a.vocab) {
         u64 n = 0;
-        row.each([&](float x) { n += x >= floor_; });
+        row.each([&](const f4v &x) { n += (x[0] >= floor_) + (x[1] >= floor_) + (x[2] >= floor_) + (x[3] >= floor_); });
         n = block_scan(n, s);
         if (t == kThreads - 1) s.before = n;
         __syncthreads();
@@ -372,13 +392,29 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
         }
         cut = s.index;
     }
-    // the draw: sums of every wave's turns, in the order of indices
-    auto turn_sum = [&](const f4v &v, int j) -> u64 {
-        u64 w = 0;
+    // The draw: sums of every wave's turns, in the order of indices.  Of a turn's 256 logits few stay behind a
+    // filter: they are gathered first, and their weights taken 64 at a time (in the wave's share of the bins).
+    float *mine = reinterpret_cast<float *>(s.bins) + 256 * wave;
+    static_assert(sizeof(s.bins) >= 4 * 256 * kWaves, "a turn of every wave");
+    auto stays = [&](const f4v &v, int j, int e) { return v[e] > last || (v[e] == last && row.index(j) + e <= cut); };
+    auto turn_sum = [&](const f4v &v, int j) -> u64 {        // the wave's, in its last lane
+        int n = 0;
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (v[e] > last || (v[e] == last && row.index(j) + e <= cut)) w += weight(v[e]);
-        return w;
+        for (int e = 0; e < 4; e++) {
+            const bool in = stays(v, j, e);
+            const u64 mask = __ballot(in);
+            if (in) mine[n + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0))] = v[e];
+            n += __popcll(mask);
+        }
+        __builtin_amdgcn_wave_barrier();                     // (a wave's accesses to shared memory are in order)
+        u64 w = 0;
+        for (int k0 = lane; k0 < n; k0 += 128) {             // two at a time
+            const float x0 = mine[k0], x1 = mine[min(k0 + 64, 255)];
+            const u64 w0 = weight(x0), w1 = weight(x1);
+            w += w0 + (k0 + 64 < n ? w1 : 0);
+        }
+        __builtin_amdgcn_wave_barrier();
+        return n ? wave_scan(w) : 0;
     };
     constexpr int AHEAD = decltype(row)::AHEAD;
     for (int j0 = 0; j0 < row.turns; j0 += AHEAD) {
@@ -388,8 +424,7 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) {
             if (j0 + j >= row.turns) continue;
-            const u64 mine = turn_sum(v[j], j0 + j);
-            const u64 upto = __any(mine != 0) ? wave_scan(mine) : 0;
+            const u64 upto = turn_sum(v[j], j0 + j);
             if (lane == 63) s.block_sum[(j0 + j) * kWaves + wave] = upto;
         }
     }
@@ -406,13 +441,16 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     const int block = s.bin, j = block / kWaves;
     if (wave == block % kWaves) {
         const f4v v = row.get(j);
-        const u64 mine = turn_sum(v, j);
-        u64 c = s.sum + wave_scan(mine) - mine;
-        if (c <= target && target < c + mine) {
+        u64 w = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (stays(v, j, e)) w += weight(v[e]);
+        u64 c = s.sum + wave_scan(w) - w;
+        if (c <= target && target < c + w) {
             bool done = false;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if (v[e] > last || (v[e] == last && row.index(j) + e <= cut)) c += weight(v[e]);
+                if (stays(v, j, e)) c += weight(v[e]);
                 if (!done && c > target) { a.token[r] = row.index(j) + e; done = true; }
             }
         }

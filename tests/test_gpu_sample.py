@@ -119,6 +119,19 @@ def test_temperatures_that_choose():
     compare(x, temperature=[1e30, 3e38] * 4, u=np.linspace(0, 0.99, 8))
 
 
+@pytest.mark.parametrize("unit", [1.4e-45, 3e-42, 1e-36, 1e-25, 1e33])
+def test_logits_of_any_size(unit):
+    """Subnormal logits, and differences that overflow: the order is that of the values all the same."""
+    rng = np.random.default_rng(6)
+    with np.errstate(under="ignore"):
+        x = (rng.integers(-300, 300, (6, 5000)).astype(np.float64) * unit).astype(np.float32)
+    x[3:, 7] = 3.3e38
+    x[3:, 8] = -3.3e38
+    t = [1.0, unit * 1e3 if unit * 1e3 > 1e-37 else 1e-37, 1e35] * 2
+    compare(x, temperature=t, top_k=[700, 5, 4000, 2, 700, 4999], u=rng.random(6))
+    compare(x, temperature=t, top_p=[0.3, 0.8, 0.5, 0.5, 0.9, 0.99], u=rng.random(6))
+
+
 @pytest.mark.parametrize("V", [1000, 32000])
 def test_equal_logits(V):
     """Whole weights: every border is met exactly, and the first of equals counts."""
