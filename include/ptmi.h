@@ -341,8 +341,9 @@ int ptmi_paged_plan_dev(const int *past, const int *fresh, int n_requests, int *
  * and value heads at k and v + r*ldkv.  rope: [rope_len][head_dim/2][2]
  * (cos, sin) of every position, for the pairs (2i, 2i+1); NULL: q and k as
  * they are (row_pos is then not read).  Rotated queries go to q_out + r*ldo,
- * which may be q; q NULL: keys and values only.  Rows whose slot lies
- * outside the cache, or whose position lies outside rope, are skipped.
+ * which may be q (with ldo = ldq); q NULL: keys and values only.  Rows whose
+ * slot lies outside the cache, or whose position lies outside rope, are
+ * skipped.
  * bf16 pages get values rounded to nearest even.  Two rows of one slot
  * leave either's there.                                                  */
 int ptmi_paged_store_dev(const ptmi_pages_t *pages, const float *q, long ldq, float *q_out, long ldo, int n_heads,
@@ -399,7 +400,8 @@ int ptmi_sample_dev(const float *logits, long ld, int rows, int vocab, const flo
  * step.  It holds the weights of m's blob, not m itself.  Continuous
  * batching of pt_generate's loop (pitorch/text/pt_text.c:314-361): prompts
  * (whole or in pieces) and single tokens share a step, requests come and go.
- * At most 2^20 rows a step and 8192 requests.                           */
+ * At most 2^20 rows a step and 8192 requests, and a vocabulary that
+ * ptmi_sample_dev takes.                                                */
 typedef struct ptmi_batch ptmi_batch_t;
 /* Host arrays by request, as ptmi_sample_dev takes them by row; NULL = off,
  * without temperature the choice is greedy.                             */

@@ -356,7 +356,7 @@ class Batch:
 
     def __init__(self, model, max_requests, max_rows, n_pages, page_size=16, cache_type=F32):
         self.L = load_ptmi()
-        self.blob = model.blob             # held: the weights' registration goes by its address
+        self.blob = model.blob             # held: the weights are registered by its address
         self.max_requests, self.vocab = max_requests, model.vocab
         h = _vp()
         check(self.L.ptmi_batch_create(model.h, max_requests, max_rows, n_pages, page_size, cache_type, ctypes.byref(h)))
@@ -377,6 +377,8 @@ class Batch:
         """new: {request: its tokens, or None: it has ended}; the parameters by request (max_requests values).
         Returns {request: next token} of those with tokens."""
         n_new, tokens = np.zeros(self.max_requests, np.int32), []
+        if any(not 0 <= r < self.max_requests for r in new):
+            raise ValueError(f"requests are 0..{self.max_requests - 1}")
         for r in sorted(new):
             n_new[r] = -1 if new[r] is None else len(new[r])
             tokens += [] if new[r] is None else list(new[r])

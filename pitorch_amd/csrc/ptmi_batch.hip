@@ -73,7 +73,7 @@ using namespace ptmi;
 
 namespace {
 
-int pages_for(int len, int page) { return (len + page - 1) / page; }
+int pages_for(int len, int page) { return len / page + (len % page != 0); }
 
 // The layers over rows [0, R) of the step: logits of `n_last` rows into b->logits.
 int enqueue_layers(ptmi_batch *b, int R, int max_new, int n_last, hipStream_t s) {
@@ -141,12 +141,15 @@ int ptmi_batch_create(ptmi_model_t *m, int max_requests, int max_rows, int n_pag
         (long long)n_pages * page_size > INT32_MAX || (cache_type != PTMI_F32 && cache_type != PTMI_BF16))
         return set_error(PTMI_ERR_ARG, "ptmi_batch_create: max_requests=%d max_rows=%d n_pages=%d page_size=%d cache_type=%d",
                          max_requests, max_rows, n_pages, page_size, cache_type);
-    int st = PTMI_OK;
-    // The batch holds the weights itself: it does not need the model any more.
-    Resident *r = register_blob(m->res->blob, m->res->bytes, false, &st);
-    if (!r) return st;
+    if (m->c.vocab > kSampleVocab)
+        return set_error(PTMI_ERR_ARG, "ptmi_batch_create: vocab=%d (at most %d)", m->c.vocab, kSampleVocab);
+    int st = ensure_init();
+    if (st) return st;
+    DeviceScope dev;
+    if ((st = dev.enter())) return st;
     ptmi_batch *b = new ptmi_batch();
-    b->res = r;
+    b->res = m->res;
+    b->res->model_holds++;           // it holds the weights itself, and needs neither the model nor the blob any more
     b->c = m->c;
     const Config &c = b->c;
     b->S = max_requests;

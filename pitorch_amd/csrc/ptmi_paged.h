@@ -36,6 +36,8 @@ struct DeviceScope {
     ~DeviceScope() { if (before >= 0) (void)hipSetDevice(before); }
 };
 
+constexpr int kSampleVocab = (1 << 18) - 4;                 // the longest row of logits a token is sampled from
+
 // PTMI_OK if the description of a paged cache is sound (host arithmetic).
 int check_pages(const char *who, const ptmi_pages_t *pages);
 

@@ -20,10 +20,11 @@ namespace {
 // lengths; for many, workgroups that each hold all sums share the rows and
 // pages (k_paged_plan), and a launch behind them writes the lengths, which
 // may stand where the cached lengths were read (k_paged_plan_end).
-// 16 requests of one token: 14.6 -> 5 us a call (sums of 1024 in 20 steps
+// 16 requests of one token: 14.6 -> 4.9 us a call (sums of 1024 in 20 steps
 // with a barrier each before, now in two); 1021 requests, 44 thousand rows,
-// 14 thousand pages: 150 -> 9 us (one workgroup, a request's pages and rows by
-// one thread each before).  Both are latency: a handful of dependent loads.
+// 14 thousand pages: 150 -> 12.4 us, 9 and 3.8 of them the two launches (one
+// workgroup, a request's pages and rows by one thread each before).  Both are
+// latency: a handful of dependent loads, and 0.4 MB written in the second.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSmall = 1024, kPlanMost = 8192;          // requests whose sums fit in shared memory
 constexpr int kPlanOneRows = 4096;                          // rows that one workgroup writes
@@ -220,7 +221,11 @@ __device__ __forceinline__ void put4(void *base, long at, float4 x) {
     }
 }
 
-// One thread per float4 of a row's [q | k | v] heads.
+// One thread per float4 of a row's [q | k | v] heads: both halves of two pairs
+// of RoPE, and nothing is read twice but the row's angles (from the caches, by
+// its heads).  Bound by the bytes: 8190 rows of 32 + 8 + 8 heads of 128, bf16
+// pages, 373 MB in 70 us, 5.3 TB/s (a large copy: 5.2); 64 rows of 12 + 12 +
+// 12 heads of 64: 3 us, the latency of a slot, a row and a store.
 template <bool BF16>
 __global__ __launch_bounds__(256) void k_paged_store(StoreArgs a) {
     const int r = blockIdx.y, slot = a.slot[r];
@@ -321,6 +326,8 @@ int ptmi_paged_store_dev(const ptmi_pages_t *pages, const float *q, long ldq, fl
         (q && (ldq % 4 || ldo % 4 || ldq < qw || ldo < qw)) || ldkv % 4 || ldkv < kw)
         return set_error(PTMI_ERR_ARG, "ptmi_paged_store: rows must be 16-byte aligned and hold their heads (ldq=%ld ldo=%ld ldkv=%ld)",
                          ldq, ldo, ldkv);
+    if (q && q_out == q && ldo != ldq)                       // (a row would be written over another)
+        return set_error(PTMI_ERR_ARG, "ptmi_paged_store: q_out is q, with another row stride (ldq=%ld ldo=%ld)", ldq, ldo);
     if ((st = ensure_init())) return st;
     DeviceScope dev;
     if ((st = dev.enter())) return st;

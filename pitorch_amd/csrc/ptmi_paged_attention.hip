@@ -6,9 +6,13 @@
 //   m' = max(m, s), l' = l 2^(m - m') + sum 2^(s - m'), o' = o 2^(m - m') + sum 2^(s - m') v
 // with scores s = (scale log2(e) q).k, so that every e^x is one 2^x.
 //
-// Two kernels, by M.  Up to 16 rows (single tokens, a few tokens) are bound
-// by the bytes of the cache: k_attn_few streams them through the fp32 matrix
-// instructions.  More rows are bound by the products: k_attn_tile.
+// Three kernels, by M.  Up to 16 rows (single tokens, a few tokens) are bound
+// by the bytes of the cache: k_attn_stream for up to 4, on the vector units,
+// k_attn_few through the fp32 matrix instructions.  More rows are bound by the
+// products: k_attn_tile, on the 16-bit matrix cores.  Against the simple form
+// (a wave a row, a key at a time): 64 requests of one token and 12 heads of 64,
+// 617 -> 40 us; 2 of 70 to 131 thousand positions, 32 heads on 8 of 128 in
+// bf16, 115600 -> 180; 16 chunks of 512 tokens, 12 heads of 64, 23100 -> 330.
 //
 // Lengths are known on the device alone, so the launch does not depend on
 // them: the work of all requests is one axis of units of 64 keys (request by
@@ -306,7 +310,9 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // index in any order that q and k share (lane group g takes float4s g, g+4,
 // ...), and the rows of V^T too: lane li loads float4s li, li+16 of a value
 // row, whose component e is row li of result tile e.  So K and V both come as
-// 16-byte loads of whole rows.
+// 16-byte loads of whole rows.  16 rows is what one such tile holds, and what
+// the bytes pay for: 64 requests of 8 new tokens, 12 heads of 64 behind up to
+// 2048 positions: 90 us, 4.5 TB/s.
 __device__ __forceinline__ f4v mfma4(float a, float b, f4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
@@ -510,8 +516,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_few(AttnArgs a) {
 // products.  Lane (g, li) of a wave takes keys 4g..4g+3 of 16 and float4s of
 // their rows: 16 lanes read a whole row of K or V side by side.  Scores are
 // summed over the 16 lanes; each lane group keeps a maximum and sums of its
-// own, and all 16 of the block's meet at the end.  64 requests of 12 heads x
-// 64, 180 MB of fp32: 55 us through the matrix instructions.
+// own, and all 16 of the block's meet at the end.  Bound by the bytes of the
+// cache: 64 requests of 12 heads of 64, 180 MB of fp32 in 35.5 us, 5.1 TB/s (55
+// us through the matrix instructions); 954 MB of bf16, 4 heads of 128 on each
+// key head: 172 us, 5.5 TB/s.
 constexpr float kLazyFew = 8.0f;     // a maximum up to 2^8 above m does not move m
 
 // FAST: four keys from a multiple of 4 on share a page, and bf16 rows may be
@@ -747,6 +755,14 @@ __global__ __launch_bounds__(kThreads) void k_attn_stream(AttnArgs a) {
 // of 2^-39 of it.  Three v_mfma_f32_32x32x16_f16 per product run at a third of
 // 1180 TFLOP/s (what a large fp16 product reaches here), the fp32 matrix
 // instructions at 154.  bf16 keys and values are h alone: two products.
+// 16 chunks of 512 behind up to 3584 positions, 12 heads of 64: 300 us, 210
+// TFLOP/s of the 390 that three products allow (bf16, 8 chunks behind 2048, 32
+// heads on 8 of 128: 370 of 590).  What bounds it is the issue of both kinds of
+// instruction: 48 matrix and some 480 vector ones (split, softmax, addresses)
+// per 64 keys of a wave's 32 rows hardly overlap, and under both the clock
+// falls to 1.55 GHz.  Measured and left: 8 waves a workgroup for heads up to 64
+// (370 us to 350 then), three waves a SIMD (453, spills), wave priorities and
+// scheduling groups (no difference).
 //
 // Wave w holds rows 32w.. of the tile as columns: S^T = K.Q^T leaves a lane
 // with 32 of the unit's scores of its row l%32 and its partner l^32 with the
@@ -1195,6 +1211,8 @@ __global__ __launch_bounds__(64 * tile_waves(DT), 2) void k_attn_tile(AttnArgs a
 }
 
 // ── joining parts ────────────────────────────────────────────────────────
+// Reads what the cut items left: 5 us behind k_attn_stream (latency), 15 behind
+// 512 workgroups of k_attn_tile, each of whose two parts is 34 KB (head_dim 64).
 // A running (m, l, o) over parts.
 struct Join {
     float m, l;

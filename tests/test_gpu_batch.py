@@ -166,6 +166,26 @@ def test_bad_batches():
         with pytest.raises(PtmiError) as e:
             pa.Batch(model, *args)
         assert e.value.status == 1
+    with pytest.raises(PtmiError) as e:
+        pa.Batch(pa.Model(pa.synth_model((8, 8, 1, 1, 1, 262141, 4), 1)), 1, 1, 1)
+    assert e.value.status == 1
+    b = pa.Batch(model, 2, 4, 4)
+    for request in (-1, 2):
+        with pytest.raises(ValueError):
+            b.step({request: [1]})
+    assert b.free_pages() == 4
+
+
+def test_the_blob_is_not_read_again():
+    """A batch takes the model's weights as they are on the GPU: the host's may be gone, and the model too."""
+    blob = pa.synth_model(SMALL, 9)
+    model = pa.Model(blob)
+    want = alone(model, [1, 2, 3], 2)[0]
+    blob[:] = 0
+    b = pa.Batch(model, 1, 8, 8)
+    model.close()
+    t = b.step({0: [1, 2, 3]})[0]
+    assert [t, b.step({0: [t]})[0]] == want
 
 
 def test_the_longest_request():

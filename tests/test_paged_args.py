@@ -59,7 +59,7 @@ def test_null_cache():
 
 @pytest.mark.parametrize("bad", [dict(rows=-1), dict(heads=0), dict(k=None), dict(v=None), dict(slot=None), dict(pos=None),
                                  dict(q_out=None), dict(rope_len=0), dict(ldq=252), dict(ldq=258), dict(ldo=128),
-                                 dict(ldkv=124), dict(q=P + 4), dict(rope=P + 8), dict(k=P + 4)], ids=str)
+                                 dict(ldkv=124), dict(q=P + 4), dict(rope=P + 8), dict(k=P + 4), dict(ldo=260)], ids=str)
 def test_store_refuses(bad):
     assert store(cache(), **bad) == ARG
 
