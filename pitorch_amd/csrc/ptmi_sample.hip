@@ -24,6 +24,7 @@
 #include "ptmi_paged.h"
 
 #include <cfloat>
+#include <climits>
 
 namespace ptmi {
 
@@ -107,8 +108,15 @@ __device__ __forceinline__ u64 wave_scan(u64 v) {          // inclusive
     return dpp_add<0x143, 0xC>(v);
 }
 
+__device__ __forceinline__ u64 last_lane(u64 v) {
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 struct SampleLds {
-    u64 bins[kBins];
+    union {
+        u64 bins[kBins];
+        float queue[kWaves][128];    // of the draw
+    };
     u64 wave[kWaves];
     float list_x[kList];
     u64 list_w[kList];
@@ -116,7 +124,7 @@ struct SampleLds {
     int members, bin, index;
     u64 before, sum;
     float value;
-    u64 block_sum[kThreads];         // sums of 256 consecutive logits' weights
+    u64 turn_sum[64];
 };
 
 // Floats as integers in the same order (-0 below 0).
@@ -140,46 +148,52 @@ __device__ __forceinline__ u64 block_scan(u64 v, SampleLds &s) {
 }
 
 // ── a row ────────────────────────────────────────────────────────────────
-// The row's logits in float4s of 16 aligned bytes; in turn j thread t has
-// float4 t + 1024 j.  What stands before and behind the row in its first and
-// last float4 counts as -infinity, as NaN does; among infinite maxima only
-// they count, as 0.  LOCAL: `at` is a copy in shared memory, else the row.
+// The row's logits in float4s of 16 aligned bytes: wave w has a run of 64
+// `turns` of them, and in turn j its lane l float4 64 (w turns + j) + l.  What
+// stands before and behind the row in its first and last float4 counts as
+// -infinity, as NaN does; among infinite maxima only they count, as 0.  LOCAL:
+// `at` is a copy in shared memory, else the row.
 template <bool LOCAL>
 struct Row {
     static constexpr int AHEAD = LOCAL ? 1 : 4;            // turns whose loads are on their way at once
     const f4v *at;
-    int skip, vocab, turns;          // floats before the row in its first float4; float4s of a thread
+    int wave, skip, vocab, turns;    // skip: floats before the row in its first float4
     bool top_inf;
 
-    __device__ __forceinline__ int index(int j) const { return 4 * ((int)threadIdx.x + kThreads * j) - skip; }
-    __device__ __forceinline__ f4v fetch(int j) const {    // from memory
-        const int i = index(j);
+    __device__ __forceinline__ int place(int w, int j) const { return (w * turns + j) * 64 + ((int)threadIdx.x & 63); }
+    __device__ __forceinline__ int index(int q) const { return 4 * q - skip; }       // of float4 q's first logit
+    __device__ __forceinline__ f4v fetch(int w, int j) const {                       // from memory
+        const int q = place(w, j), q0 = (w * turns + j) * 64;
         f4v v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (i < vocab) {
-            v = at[threadIdx.x + kThreads * j];
+        if (index(q0) >= 0 && index(q0 + 64) <= vocab) {                             // uniform: all inside
+            v = at[q];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = fmaxf(v[e] + 0.0f, -INFINITY);        // (-0 as 0, NaN as -infinity)
+        } else if (index(q) < vocab) {
+            const f4v x = at[q];
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                v[e] = (unsigned)(i + e) < (unsigned)vocab && v[e] > -INFINITY ? v[e] + 0.0f : -INFINITY;   // (-0 as 0)
+                if ((unsigned)(index(q) + e) < (unsigned)vocab) v[e] = fmaxf(x[e] + 0.0f, -INFINITY);
         }
         return v;
     }
-    __device__ __forceinline__ f4v get(int j) const {
-        f4v v = LOCAL ? at[threadIdx.x + kThreads * j] : fetch(j);
+    __device__ __forceinline__ f4v get(int w, int j) const {
+        f4v v = LOCAL ? at[place(w, j)] : fetch(w, j);
         if (top_inf)
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = v[e] == INFINITY ? 0.0f : -INFINITY;
         return v;
     }
-    // f(four logits) for all of this thread's: four at a time, because a weight is a chain of dependent operations
+    // f(four logits, their place) for all of this thread's
     template <typename F>
     __device__ __forceinline__ void each(F &&f) const {
         for (int j0 = 0; j0 < turns; j0 += AHEAD) {
             f4v v[AHEAD];
 #pragma unroll
-            for (int j = 0; j < AHEAD; j++) v[j] = get(min(j0 + j, turns - 1));
+            for (int j = 0; j < AHEAD; j++) v[j] = get(wave, min(j0 + j, turns - 1));
 #pragma unroll
             for (int j = 0; j < AHEAD; j++)
-                if (j0 + j < turns) f(v[j]);
+                if (j0 + j < turns) f(v[j], place(wave, j0 + j));
         }
     }
 };
@@ -194,12 +208,12 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
     const int t = threadIdx.x;
     Mark k = {hi, 0, 0, 0};
     bool first = true;
-    for (;;) {
+    for (int step = 0; step < 64; step++) {                  // (each takes 11 bits of the bounds' distance: under 40)
         // Bins of (hi - x)/2, which no pair of floats overflows.  lo < hi fall into different ones, so the bounds
         // close in; where even half their distance is nothing (subnormals next to each other), hi alone is a bin.
         const float half = 0.5f * hi, range = half - 0.5f * lo;
-        const bool apart = range > 0.0f;
-        const float pre = range < 1e-20f ? 0x1p100f : 1.0f, inv = apart ? (float)kBins / (range * pre) : 0.0f;   // (finite)
+        const bool apart = range > 0.0f, normal = range >= 1e-20f;
+        const float pre = normal ? 1.0f : 0x1p100f, inv = apart ? (float)kBins / (range * pre) : 0.0f;   // (finite)
         auto bin_of = [&](float x) {
             const int b = min((int)(fmaf(-0.5f, x, half) * pre * inv), kBins - 1);
             return apart || x == hi ? b : 1;
@@ -207,14 +221,25 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
         s.bins[t] = s.bins[t + kThreads] = 0;
         if (t == 0) { s.members = 0; s.lo = 0xFFFFFFFFu; s.hi = 0; }
         __syncthreads();
-        row.each([&](const f4v &x) {
-            u64 w[4];
+        if (first && normal) {                               // (as below, but hi is the largest and pre 1)
+            row.each([&](const f4v &x, int) {
+                u64 w[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = measure(x[e]);
+                for (int e = 0; e < 4; e++) w[e] = measure(x[e]);
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (x[e] >= lo && x[e] <= hi && w[e]) atomicAdd(&s.bins[bin_of(x[e])], w[e]);
-        });
+                for (int e = 0; e < 4; e++)
+                    if (x[e] >= lo && w[e]) atomicAdd(&s.bins[min((int)(fmaf(-0.5f, x[e], half) * inv), kBins - 1)], w[e]);
+            });
+        } else {
+            row.each([&](const f4v &x, int) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (!(x[e] >= lo && x[e] <= hi)) continue;
+                    const u64 w = measure(x[e]);
+                    if (w) atomicAdd(&s.bins[bin_of(x[e])], w);
+                }
+            });
+        }
         __syncthreads();
         const u64 b0 = s.bins[2 * t], b1 = s.bins[2 * t + 1], c1 = block_scan(b0 + b1, s), c0 = c1 - b1, cb = c0 - b0;
         if (first) {
@@ -232,12 +257,23 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
         k.equals = s.sum;
         k.value = hi;
         if (!(lo < hi)) { __syncthreads(); return k; }      // all equal
+        // Bounds a little outside of the bin's (its border is off by a few roundings of bin/inv and of hi) spare most
+        // logits the rest.  In halves, as the bins: finite, up to `from`, which may be -infinity.
+        float from = lo, to = hi;
+        if (normal) {
+            const float width = range / kBins, off = 1e-6f * fabsf(half);
+            if (bin < kBins - 1) from = fmaxf(lo, 2.0f * (half - (float)(bin + 1) * width * 1.00001f - off));
+            to = fminf(hi, 2.0f * (half - (float)bin * width * 0.99999f + off));
+        }
         float least = INFINITY, most = -INFINITY;
-        row.each([&](const f4v &x) {
+        row.each([&](const f4v &x, int) {
+            bool some = false;
+#pragma unroll
+            for (int e = 0; e < 4; e++) some |= x[e] >= from && x[e] <= to;
+            if (!some) return;
             unsigned in = 0;
 #pragma unroll
             for (int e = 0; e < 4; e++) in |= x[e] >= lo && x[e] <= hi && bin_of(x[e]) == bin ? 1u << e : 0;
-            if (!in) return;
             for (int e = 0; e < 4; e++) {
                 if (!(in >> e & 1)) continue;
                 const float y = e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3];
@@ -281,6 +317,7 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
         }
         __syncthreads();
     }
+    return k;
 }
 
 // CAP: logits that the copy in shared memory holds; 0: no copy.  Where two
@@ -290,11 +327,12 @@ template <int CAP>
 __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_sample(SampleArgs a) {
     __shared__ SampleLds s;
     __shared__ f4v copy[CAP ? CAP / 4 : 1];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = blockIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = blockIdx.x;
     const float *logits = a.logits + (long)r * a.ld;
     Row<(CAP > 0)> row;
     row.skip = (int)((uintptr_t)logits >> 2 & 3);
     row.at = reinterpret_cast<const f4v *>(logits - row.skip);
+    row.wave = wave;
     row.vocab = a.vocab;
     row.turns = (a.vocab + row.skip + 4 * kThreads - 1) / (4 * kThreads);
     row.top_inf = false;
@@ -306,8 +344,8 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     float top = -INFINITY;
 #pragma unroll 8
     for (int j = 0; j < row.turns; j++) {
-        const f4v v = row.fetch(j);
-        if constexpr (CAP > 0) copy[t + kThreads * j] = v;   // (each thread reads back its own)
+        const f4v v = row.fetch(wave, j);
+        if constexpr (CAP > 0) copy[row.place(wave, j)] = v; // (a wave reads another's only behind a barrier)
         top = fmaxf(fmaxf(top, fmaxf(v[0], v[1])), fmaxf(v[2], v[3]));
     }
     if constexpr (CAP > 0) row.at = copy;
@@ -328,11 +366,10 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     }
     if (!(temp > 0.0f) || top_k == 1) {                      // the first index of the maximum
         int i = a.vocab;
-        for (int j = row.turns - 1; j >= 0; j--) {
-            const f4v v = row.get(j);
+        row.each([&](const f4v &v, int q) {
 #pragma unroll
-            for (int e = 3; e >= 0; e--) i = v[e] == top ? row.index(j) + e : i;
-        }
+            for (int e = 3; e >= 0; e--) i = v[e] == top ? min(i, row.index(q) + e) : i;
+        });
         for (int d = 32; d; d >>= 1) i = min(i, __shfl_xor(i, d));
         if (lane == 0) atomicMin(&s.index, i);
         __syncthreads();
@@ -349,7 +386,7 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     u64 ties = (u64)a.vocab, equals = 0;
     if (top_k > 0 && top_k < a.vocab) {
         u64 n = 0;
-        row.each([&](const f4v &x) { n += (x[0] >= floor_) + (x[1] >= floor_) + (x[2] >= floor_) + (x[3] >= floor_); });
+        row.each([&](const f4v &x, int) { n += (x[0] >= floor_) + (x[1] >= floor_) + (x[2] >= floor_) + (x[3] >= floor_); });
         n = block_scan(n, s);
         if (t == kThreads - 1) s.before = n;
         __syncthreads();
@@ -382,86 +419,106 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
         }
     }
     // more equals of the last than stay: the index of the last that does
-    int cut = a.vocab;
+    int cut = INT_MAX;
     if (equals > ties) {                                     // uniform
+        auto equal = [&](const f4v &v) { return (v[0] == last) + (v[1] == last) + (v[2] == last) + (v[3] == last); };
         u64 seen = 0;
-        for (int j = 0; j < row.turns; j++) {
-            const f4v v = row.get(j);
-            const u64 mine = (v[0] == last) + (v[1] == last) + (v[2] == last) + (v[3] == last);
-            const u64 upto = block_scan(mine, s), from = seen + upto - mine;
-            if (from < ties && ties <= from + mine) {
-                int k = (int)(ties - from);
-                for (int e = 0; e < 4; e++)
-                    if (v[e] == last && --k == 0) s.index = row.index(j) + e;
-            }
-            if (t == kThreads - 1) s.before = upto;
-            __syncthreads();
-            seen += s.before;
-            __syncthreads();
-        }
+        row.each([&](const f4v &v, int) { seen += equal(v); });
+        seen = wave_scan(seen);
+        if (lane == 63) s.wave[wave] = seen;
+        __syncthreads();
+        seen = 0;                                            // before this wave's run
+        for (int w = 0; w < wave; w++) seen += s.wave[w];
+        row.each([&](const f4v &v, int q) {
+            const u64 mine = equal(v), upto = seen + wave_scan(mine), from = upto - mine;
+            int k = (int)(ties - from), at = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (v[e] == last && --k == 0) at = e;
+            if (from < ties && ties <= upto) s.index = row.index(q) + at;
+            seen = last_lane(upto);
+        });
+        __syncthreads();
         cut = s.index;
     }
-    // The draw: sums of every wave's turns, in the order of indices.  Of a turn's 256 logits few stay behind a
-    // filter: they are gathered first, and their weights taken 64 at a time (in the wave's share of the bins).
-    float *mine = reinterpret_cast<float *>(s.bins) + 256 * wave;
-    static_assert(sizeof(s.bins) >= 4 * 256 * kWaves, "a turn of every wave");
-    auto stays = [&](const f4v &v, int j, int e) { return v[e] > last || (v[e] == last && row.index(j) + e <= cut); };
-    auto turn_sum = [&](const f4v &v, int j) -> u64 {        // the wave's, in its last lane
-        int n = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const bool in = stays(v, j, e);
-            const u64 mask = __ballot(in);
-            if (in) mine[n + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0))] = v[e];
-            n += __popcll(mask);
-        }
-        __builtin_amdgcn_wave_barrier();                     // (a wave's accesses to shared memory are in order)
+    // The draw, in the order of indices: sums of the waves' runs, then of the turns of the run that holds the mark, a
+    // turn a wave.  Behind a filter few logits stay: they are picked out first, and their weights taken 64 at a time.
+    const bool tied = cut != INT_MAX;                        // uniform, and hardly ever so
+    const float above = tied ? last : last == 0.0f ? -0x1p-149f : from_ordered(ordered(last) - 1);   // (the next float below)
+    auto stays = [&](float x, int i) { return x > above || (tied && x == last && i <= cut); };
+    {
+        // (a wave's accesses to shared memory are in order)
         u64 w = 0;
-        for (int k0 = lane; k0 < n; k0 += 128) {             // two at a time
-            const float x0 = mine[k0], x1 = mine[min(k0 + 64, 255)];
-            const u64 w0 = weight(x0), w1 = weight(x1);
-            w += w0 + (k0 + 64 < n ? w1 : 0);
-        }
-        __builtin_amdgcn_wave_barrier();
-        return n ? wave_scan(w) : 0;
-    };
-    constexpr int AHEAD = decltype(row)::AHEAD;
-    for (int j0 = 0; j0 < row.turns; j0 += AHEAD) {
-        f4v v[AHEAD];
-#pragma unroll
-        for (int j = 0; j < AHEAD; j++) v[j] = row.get(min(j0 + j, row.turns - 1));
-#pragma unroll
-        for (int j = 0; j < AHEAD; j++) {
-            if (j0 + j >= row.turns) continue;
-            const u64 upto = turn_sum(v[j], j0 + j);
-            if (lane == 63) s.block_sum[(j0 + j) * kWaves + wave] = upto;
-        }
-    }
-    __syncthreads();
-    const int blocks = row.turns * kWaves;                   // at most kThreads
-    const u64 one = t < blocks ? s.block_sum[t] : 0, upto = block_scan(one, s);
-    if (t == kThreads - 1) s.before = upto;
-    __syncthreads();
-    const u64 total = s.before;
-    u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
-    const u64 target = min((u64)((double)u * (double)total), total - 1);
-    if (upto - one <= target && target < upto) { s.bin = t; s.sum = upto - one; }
-    __syncthreads();
-    const int block = s.bin, j = block / kWaves;
-    if (wave == block % kWaves) {
-        const f4v v = row.get(j);
-        u64 w = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (stays(v, j, e)) w += weight(v[e]);
-        u64 c = s.sum + wave_scan(w) - w;
-        if (c <= target && target < c + w) {
-            bool done = false;
+        int n = 0;                                           // in the wave's queue, under 64 between turns of the loop
+        row.each([&](const f4v &v, int q) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                if (stays(v, j, e)) c += weight(v[e]);
-                if (!done && c > target) { a.token[r] = row.index(j) + e; done = true; }
+                const bool in = stays(v[e], row.index(q) + e);
+                const u64 mask = __ballot(in);
+                if (!mask) continue;
+                if (in) s.queue[wave][n + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0))] = v[e];
+                n += __popcll(mask);
+                __builtin_amdgcn_wave_barrier();
+                if (n < 64) continue;
+                w += weight(s.queue[wave][lane]);
+                n -= 64;
+                const float rest = s.queue[wave][64 + lane];
+                __builtin_amdgcn_wave_barrier();
+                s.queue[wave][lane] = rest;                  // (past n: not used)
+                __builtin_amdgcn_wave_barrier();
             }
+        });
+        if (n > 0) {
+            const u64 one = weight(s.queue[wave][min(lane, n - 1)]);
+            w += lane < n ? one : 0;
+        }
+        w = wave_scan(w);
+        if (lane == 63) s.wave[wave] = w;
+    }
+    __syncthreads();
+    u64 total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) total += s.wave[w];
+    u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+    const u64 target = min((u64)((double)u * (double)total), total - 1);
+    u64 before = 0, sum = 0;
+    int run = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        const u64 upto = sum + s.wave[w];
+        if (sum <= target && target < upto) { run = w; before = sum; }
+        sum = upto;
+    }
+    run = __builtin_amdgcn_readfirstlane(run);
+    f4v v;
+    auto four = [&](int j) -> u64 {                          // this lane's weights of turn j of the run
+        v = row.get(run, j);
+        u64 w = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const u64 one = weight(v[e]);
+            w += stays(v[e], row.index(row.place(run, j)) + e) ? one : 0;
+        }
+        return w;
+    };
+    for (int j = wave; j < row.turns; j += kWaves) {
+        const u64 upto = wave_scan(four(j));
+        if (lane == 63) s.turn_sum[j] = upto;
+    }
+    __syncthreads();
+    const u64 mine = lane < row.turns ? s.turn_sum[lane] : 0, upto = before + wave_scan(mine), past = __ballot(upto > target);
+    if (!past) return;                                       // (never: the run holds the mark)
+    const int j = __ffsll((unsigned long long)past) - 1;
+    if (wave != j % kWaves) return;
+    const u64 w = four(j);
+    u64 c = __shfl(upto - mine, j) + wave_scan(w) - w;
+    if (c <= target && target < c + w) {
+        bool done = false;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int i = row.index(row.place(run, j)) + e;
+            if (stays(v[e], i)) c += weight(v[e]);
+            if (!done && c > target) { a.token[r] = i; done = true; }
         }
     }
 }
