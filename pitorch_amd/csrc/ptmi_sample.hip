@@ -35,7 +35,7 @@ typedef float f4v __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2 * kThreads;
-constexpr int kList = 128;           // logits of a bin that are compared with each other
+constexpr int kList = 256;           // logits of a bin that are compared with each other, by kThreads / kList threads each
 static_assert(kSampleVocab <= 64 * 4 * kThreads - 4, "64 turns of a block, wherever in a float4 a row starts");
 
 struct SampleArgs {
@@ -108,18 +108,21 @@ __device__ __forceinline__ u64 wave_scan(u64 v) {          // inclusive
     return dpp_add<0x143, 0xC>(v);
 }
 
-__device__ __forceinline__ u64 last_lane(u64 v) {
-    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+// Lane i's value, i the same in all lanes.
+__device__ __forceinline__ u64 lane_value(u64 v, int i) {
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)v, i);
 }
+
+constexpr int kQueue = 64 + 4 * 64;  // logits a wave has picked out: under 64, and what its next turn adds
 
 struct SampleLds {
     union {
         u64 bins[kBins];
-        float queue[kWaves][128];    // of the draw
+        float queue[kWaves][kQueue]; // of the draw
     };
     u64 wave[kWaves];
     float list_x[kList];
-    u64 list_w[kList];
+    u64 list_w[kList], above[kList], equal[kList];
     unsigned lo, hi;                 // of a bin's members, as ordered bits
     int members, bin, index;
     u64 before, sum;
@@ -136,18 +139,22 @@ __device__ __forceinline__ float from_ordered(unsigned k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// Inclusive sums over the block.
-__device__ __forceinline__ u64 block_scan(u64 v, SampleLds &s) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    v = wave_scan(v);
-    if (lane == 63) s.wave[w] = v;
+// Sums over the waves, from every wave's sums over its lanes: lane w gets that of waves 0..w, from 15 on the whole
+// one.  (s.wave is not to be written again before another barrier.)
+__device__ __forceinline__ u64 sum_waves(u64 scanned, SampleLds &s, int wave) {
+    const int lane = threadIdx.x & 63;
+    if (lane == 63) s.wave[wave] = scanned;
     __syncthreads();
-    for (int i = 0; i < w; i++) v += s.wave[i];
-    __syncthreads();
-    return v;
+    return wave_scan(lane < kWaves ? s.wave[lane] : 0);
 }
 
 // ── a row ────────────────────────────────────────────────────────────────
+__device__ __forceinline__ f4v only_infinite(f4v v) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = v[e] == INFINITY ? 0.0f : -INFINITY;
+    return v;
+}
+
 // The row's logits in float4s of 16 aligned bytes: wave w has a run of 64
 // `turns` of them, and in turn j its lane l float4 64 (w turns + j) + l.  What
 // stands before and behind the row in its first and last float4 counts as
@@ -178,10 +185,12 @@ struct Row {
         return v;
     }
     __device__ __forceinline__ f4v get(int w, int j) const {
-        f4v v = LOCAL ? at[place(w, j)] : fetch(w, j);
-        if (top_inf)
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = v[e] == INFINITY ? 0.0f : -INFINITY;
+        if constexpr (LOCAL) return at[place(w, j)];
+        f4v v = fetch(w, j);
+        if (top_inf) {
+            asm("");                                         // (a branch, not six more instructions for every four)
+            v = only_infinite(v);
+        }
         return v;
     }
     // f(four logits, their place) for all of this thread's
@@ -201,10 +210,11 @@ struct Row {
 // The logit at which the running sum of `measure` over the logits in [lo, hi],
 // in their order, reaches need(their whole sum), which is more than 0 and at
 // most that sum: its value, the sum before it and the sum of its equals.
+// many: logits in the bounds are no exception.
 struct Mark { float value; u64 before, equals, need; };
 
 template <bool LOCAL, typename M, typename F>
-__device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float hi, const M &measure, F &&need_of) {
+__device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float hi, bool many, const M &measure, F &&need_of) {
     const int t = threadIdx.x;
     Mark k = {hi, 0, 0, 0};
     bool first = true;
@@ -219,9 +229,10 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
             return apart || x == hi ? b : 1;
         };
         s.bins[t] = s.bins[t + kThreads] = 0;
+        if (t < kList) s.above[t] = s.equal[t] = 0;
         if (t == 0) { s.members = 0; s.lo = 0xFFFFFFFFu; s.hi = 0; }
         __syncthreads();
-        if (first && normal) {                               // (as below, but hi is the largest and pre 1)
+        if (first && normal && many) {                       // (as below, but hi is the largest and pre 1)
             row.each([&](const f4v &x, int) {
                 u64 w[4];
 #pragma unroll
@@ -241,14 +252,10 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
             });
         }
         __syncthreads();
-        const u64 b0 = s.bins[2 * t], b1 = s.bins[2 * t + 1], c1 = block_scan(b0 + b1, s), c0 = c1 - b1, cb = c0 - b0;
-        if (first) {
-            if (t == kThreads - 1) s.before = c1;
-            __syncthreads();
-            k.need = need_of(s.before);
-            __syncthreads();
-            first = false;
-        }
+        const u64 b0 = s.bins[2 * t], b1 = s.bins[2 * t + 1], scanned = wave_scan(b0 + b1), sums = sum_waves(scanned, s, row.wave);
+        const u64 c1 = scanned + (row.wave ? lane_value(sums, row.wave - 1) : 0), c0 = c1 - b1, cb = c0 - b0;
+        if (first) k.need = need_of(lane_value(sums, 63));
+        first = false;
         if (k.before + cb < k.need && k.need <= k.before + c0) { s.bin = 2 * t; s.before = k.before + cb; s.sum = b0; }
         if (k.before + c0 < k.need && k.need <= k.before + c1) { s.bin = 2 * t + 1; s.before = k.before + c0; s.sum = b1; }
         __syncthreads();
@@ -256,7 +263,7 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
         k.before = s.before;
         k.equals = s.sum;
         k.value = hi;
-        if (!(lo < hi)) { __syncthreads(); return k; }      // all equal
+        if (!(lo < hi)) return k;                            // all equal
         // Bounds a little outside of the bin's (its border is off by a few roundings of bin/inv and of hi) spare most
         // logits the rest.  In halves, as the bins: finite, up to `from`, which may be -infinity.
         float from = lo, to = hi;
@@ -297,22 +304,28 @@ __device__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float h
         lo = from_ordered(s.lo);
         hi = from_ordered(s.hi);
         if (n <= kList) {
-            if (t < n) {
-                const float x = s.list_x[t];
-                u64 above = k.before, equal = 0;
-                for (int i = 0; i < n; i++) {
-                    const float y = s.list_x[i];
-                    const u64 w = s.list_w[i];
+            const int i = t % kList;
+            if (i < n) {
+                const float x = s.list_x[i];
+                u64 above = 0, equal = 0;
+                for (int j = t / kList; j < n; j += kThreads / kList) {
+                    const float y = s.list_x[j];
+                    const u64 w = s.list_w[j];
                     above += y > x ? w : 0;
                     equal += y == x ? w : 0;
                 }
-                if (above < k.need && k.need <= above + equal) { s.value = x; s.before = above; s.sum = equal; }   // equals agree
+                if (above) atomicAdd(&s.above[i], above);
+                if (equal) atomicAdd(&s.equal[i], equal);
+            }
+            __syncthreads();
+            if (t < n) {
+                const u64 above = k.before + s.above[t], equal = s.equal[t];
+                if (above < k.need && k.need <= above + equal) { s.value = s.list_x[t]; s.before = above; s.sum = equal; }   // equals agree
             }
             __syncthreads();
             k.value = s.value;
             k.before = s.before;
             k.equals = s.sum;
-            __syncthreads();
             return k;
         }
         __syncthreads();
@@ -355,7 +368,6 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWaves; w++) top = fmaxf(top, s.list_x[w]);
-    __syncthreads();
     if (top == -INFINITY) {
         if (t == 0) a.token[r] = -1;
         return;
@@ -363,6 +375,8 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     if (top == INFINITY) {                                   // uniform
         row.top_inf = true;
         top = 0.0f;
+        if constexpr (CAP > 0)
+            for (int j = 0; j < row.turns; j++) copy[row.place(wave, j)] = only_infinite(copy[row.place(wave, j)]);
     }
     if (!(temp > 0.0f) || top_k == 1) {                      // the first index of the maximum
         int i = a.vocab;
@@ -385,24 +399,15 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     float last = floor_;
     u64 ties = (u64)a.vocab, equals = 0;
     if (top_k > 0 && top_k < a.vocab) {
-        u64 n = 0;
-        row.each([&](const f4v &x, int) { n += (x[0] >= floor_) + (x[1] >= floor_) + (x[2] >= floor_) + (x[3] >= floor_); });
-        n = block_scan(n, s);
-        if (t == kThreads - 1) s.before = n;
-        __syncthreads();
-        const bool fewer = (u64)top_k < s.before;            // uniform: top_k leaves out some that weigh
-        __syncthreads();
-        if (fewer) {
-            const Mark k = find_mark(row, s, floor_, top, CountOf(), [&](u64) { return (u64)top_k; });
-            last = k.value;
-            equals = k.equals;
-            ties = (u64)top_k - k.before;
-        }
+        const Mark k = find_mark(row, s, floor_, top, true, CountOf(), [&](u64 weigh) { return min((u64)top_k, weigh); });
+        last = k.value;
+        equals = k.equals;
+        ties = k.need - k.before;
     }
     if (!(top_p >= 1.0f)) {
         const u64 dropped = equals > ties ? (equals - ties) * weight(last) : 0;
         // stays: sums before it under top_p * total, so the last is where the sum reaches it
-        const Mark k = find_mark(row, s, last, top, weight, [&](u64 sum) {
+        const Mark k = find_mark(row, s, last, top, equals == 0 || top_k > a.vocab / 32, weight, [&](u64 sum) {
             const double lim = top_p > 0.0f ? (double)top_p * (double)(sum - dropped) : 0.0;
             u64 need = (u64)lim;
             if ((double)need < lim) need++;
@@ -424,11 +429,8 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
         auto equal = [&](const f4v &v) { return (v[0] == last) + (v[1] == last) + (v[2] == last) + (v[3] == last); };
         u64 seen = 0;
         row.each([&](const f4v &v, int) { seen += equal(v); });
-        seen = wave_scan(seen);
-        if (lane == 63) s.wave[wave] = seen;
-        __syncthreads();
-        seen = 0;                                            // before this wave's run
-        for (int w = 0; w < wave; w++) seen += s.wave[w];
+        const u64 sums = sum_waves(wave_scan(seen), s, wave);
+        seen = wave ? lane_value(sums, wave - 1) : 0;        // before this wave's run
         row.each([&](const f4v &v, int q) {
             const u64 mine = equal(v), upto = seen + wave_scan(mine), from = upto - mine;
             int k = (int)(ties - from), at = 0;
@@ -436,7 +438,7 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
             for (int e = 0; e < 4; e++)
                 if (v[e] == last && --k == 0) at = e;
             if (from < ties && ties <= upto) s.index = row.index(q) + at;
-            seen = last_lane(upto);
+            seen = lane_value(upto, 63);
         });
         __syncthreads();
         cut = s.index;
@@ -446,50 +448,48 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     const bool tied = cut != INT_MAX;                        // uniform, and hardly ever so
     const float above = tied ? last : last == 0.0f ? -0x1p-149f : from_ordered(ordered(last) - 1);   // (the next float below)
     auto stays = [&](float x, int i) { return x > above || (tied && x == last && i <= cut); };
+    u64 w = 0;
     {
         // (a wave's accesses to shared memory are in order)
-        u64 w = 0;
         int n = 0;                                           // in the wave's queue, under 64 between turns of the loop
         row.each([&](const f4v &v, int q) {
+            bool in[4];
+            u64 mask[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const bool in = stays(v[e], row.index(q) + e);
-                const u64 mask = __ballot(in);
-                if (!mask) continue;
-                if (in) s.queue[wave][n + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0))] = v[e];
-                n += __popcll(mask);
-                __builtin_amdgcn_wave_barrier();
-                if (n < 64) continue;
-                w += weight(s.queue[wave][lane]);
-                n -= 64;
-                const float rest = s.queue[wave][64 + lane];
-                __builtin_amdgcn_wave_barrier();
-                s.queue[wave][lane] = rest;                  // (past n: not used)
-                __builtin_amdgcn_wave_barrier();
+                in[e] = stays(v[e], row.index(q) + e);
+                mask[e] = __ballot(in[e]);
             }
+            if (!(mask[0] | mask[1] | mask[2] | mask[3])) return;
+            if (!~(mask[0] & mask[1] & mask[2] & mask[3])) { // none to pick out
+#pragma unroll
+                for (int e = 0; e < 4; e++) w += weight(v[e]);
+                return;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int at = (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask[e] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask[e], n));
+                if (in[e]) s.queue[wave][at] = v[e];
+                n += __popcll(mask[e]);
+            }
+            __builtin_amdgcn_wave_barrier();
+            while (n >= 64) {                                // (under kQueue)
+                n -= 64;
+                w += weight(s.queue[wave][n + lane]);
+            }
+            __builtin_amdgcn_wave_barrier();
         });
         if (n > 0) {
             const u64 one = weight(s.queue[wave][min(lane, n - 1)]);
             w += lane < n ? one : 0;
         }
-        w = wave_scan(w);
-        if (lane == 63) s.wave[wave] = w;
     }
-    __syncthreads();
-    u64 total = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) total += s.wave[w];
+    w = sum_waves(wave_scan(w), s, wave);
+    const u64 total = lane_value(w, 63);
     u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
     const u64 target = min((u64)((double)u * (double)total), total - 1);
-    u64 before = 0, sum = 0;
-    int run = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) {
-        const u64 upto = sum + s.wave[w];
-        if (sum <= target && target < upto) { run = w; before = sum; }
-        sum = upto;
-    }
-    run = __builtin_amdgcn_readfirstlane(run);
+    const int run = max(__ffsll((unsigned long long)__ballot(w > target)) - 1, 0);   // (under kWaves: from lane 15 on w is total)
+    const u64 before = run > 0 ? lane_value(w, run - 1) : 0;
     f4v v;
     auto four = [&](int j) -> u64 {                          // this lane's weights of turn j of the run
         v = row.get(run, j);
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     if (!past) return;                                       // (never: the run holds the mark)
     const int j = __ffsll((unsigned long long)past) - 1;
     if (wave != j % kWaves) return;
-    const u64 w = four(j);
+    w = four(j);
     u64 c = __shfl(upto - mine, j) + wave_scan(w) - w;
     if (c <= target && target < c + w) {
         bool done = false;
