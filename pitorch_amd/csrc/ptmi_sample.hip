@@ -61,17 +61,14 @@ struct Exp2Poly {
 };
 // 2^y for y in (-1000, 0]: 2^n p(f), n the nearest integer, p of degree 9
 // through 2^f at the Chebyshev nodes of [-1/2, 1/2] (relative error 1.9e-14,
-// a third of 2^-44).  y + 1.5 2^52 has n as its last bits, and n added to
-// p's exponent bits is the product.
+// a third of 2^-44).  y + 1.5 2^52 has n as its last bits.
 __device__ __forceinline__ double exp2_weight(const Exp2Poly &q, double y) {
     constexpr double kShift = 6755399441055744.0;
     const double n = y + kShift, f = y - (n - kShift);
     double p = q.c[9];
 #pragma unroll
     for (int i = 8; i >= 0; i--) p = fma(p, f, q.c[i]);
-    const u64 bits = (u64)__double_as_longlong(p);
-    const unsigned hi = (unsigned)(bits >> 32) + ((unsigned)__double_as_longlong(n) << 20);
-    return __longlong_as_double((long long)((u64)hi << 32 | (unsigned)bits));
+    return __builtin_amdgcn_ldexp(p, (int)__double_as_longlong(n));
 }
 // To the nearest multiple of 2^-44, as their number: w + 2^8 has them as its last bits.
 __device__ __forceinline__ u64 fixed(double w) {
@@ -210,11 +207,11 @@ struct Row {
 // The logit at which the running sum of `measure` over the logits in [lo, hi],
 // in their order, reaches need(their whole sum), which is more than 0 and at
 // most that sum: its value, the sum before it and the sum of its equals.
-// many: logits in the bounds are no exception.
+// logits: how many lie in the bounds, or more.
 struct Mark { float value; u64 before, equals, need; };
 
 template <bool LOCAL, typename M, typename F>
-__device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float hi, bool many, const M &measure, F &&need_of) {
+__device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float hi, int logits, const M &measure, F &&need_of) {
     const int t = threadIdx.x;
     Mark k = {hi, 0, 0, 0};
     bool first = true;
@@ -228,46 +225,52 @@ __device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, f
             const int b = min((int)(fmaf(-0.5f, x, half) * pre * inv), kBins - 1);
             return apart || x == hi ? b : 1;
         };
-        s.bins[t] = s.bins[t + kThreads] = 0;
         if (t < kList) s.above[t] = s.equal[t] = 0;
         if (t == 0) { s.members = 0; s.lo = 0xFFFFFFFFu; s.hi = 0; }
-        __syncthreads();
-        if (first && normal && many) {                       // (as below, but hi is the largest and pre 1)
-            row.each([&](const f4v &x, int) {
-                u64 w[4];
+        int bin = -1;                                        // none: all in [lo, hi], which are few
+        if (logits > kList) {
+            s.bins[t] = s.bins[t + kThreads] = 0;
+            __syncthreads();
+            if (first && normal && logits > row.vocab / 32) {   // (as below, but hi is the largest and pre 1)
+                row.each([&](const f4v &x, int) {
+                    u64 w[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = measure(x[e]);
+                    for (int e = 0; e < 4; e++) w[e] = measure(x[e]);
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (x[e] >= lo && w[e]) atomicAdd(&s.bins[min((int)(fmaf(-0.5f, x[e], half) * inv), kBins - 1)], w[e]);
-            });
+                    for (int e = 0; e < 4; e++)
+                        if (x[e] >= lo && w[e]) atomicAdd(&s.bins[min((int)(fmaf(-0.5f, x[e], half) * inv), kBins - 1)], w[e]);
+                });
+            } else {
+                row.each([&](const f4v &x, int) {
+                    if (!__any(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) >= lo)) return;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (!(x[e] >= lo && x[e] <= hi)) continue;
+                        const u64 w = measure(x[e]);
+                        if (w) atomicAdd(&s.bins[bin_of(x[e])], w);
+                    }
+                });
+            }
+            __syncthreads();
+            const u64 b0 = s.bins[2 * t], b1 = s.bins[2 * t + 1], scanned = wave_scan(b0 + b1), sums = sum_waves(scanned, s, row.wave);
+            const u64 c1 = scanned + (row.wave ? lane_value(sums, row.wave - 1) : 0), c0 = c1 - b1, cb = c0 - b0;
+            if (first) k.need = need_of(lane_value(sums, 63));
+            first = false;
+            if (k.before + cb < k.need && k.need <= k.before + c0) { s.bin = 2 * t; s.before = k.before + cb; s.sum = b0; }
+            if (k.before + c0 < k.need && k.need <= k.before + c1) { s.bin = 2 * t + 1; s.before = k.before + c0; s.sum = b1; }
+            __syncthreads();
+            bin = s.bin;
+            k.before = s.before;
+            k.equals = s.sum;
+            k.value = hi;
+            if (!(lo < hi)) return k;                            // all equal
         } else {
-            row.each([&](const f4v &x, int) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (!(x[e] >= lo && x[e] <= hi)) continue;
-                    const u64 w = measure(x[e]);
-                    if (w) atomicAdd(&s.bins[bin_of(x[e])], w);
-                }
-            });
+            __syncthreads();
         }
-        __syncthreads();
-        const u64 b0 = s.bins[2 * t], b1 = s.bins[2 * t + 1], scanned = wave_scan(b0 + b1), sums = sum_waves(scanned, s, row.wave);
-        const u64 c1 = scanned + (row.wave ? lane_value(sums, row.wave - 1) : 0), c0 = c1 - b1, cb = c0 - b0;
-        if (first) k.need = need_of(lane_value(sums, 63));
-        first = false;
-        if (k.before + cb < k.need && k.need <= k.before + c0) { s.bin = 2 * t; s.before = k.before + cb; s.sum = b0; }
-        if (k.before + c0 < k.need && k.need <= k.before + c1) { s.bin = 2 * t + 1; s.before = k.before + c0; s.sum = b1; }
-        __syncthreads();
-        const int bin = s.bin;
-        k.before = s.before;
-        k.equals = s.sum;
-        k.value = hi;
-        if (!(lo < hi)) return k;                            // all equal
         // Bounds a little outside of the bin's (its border is off by a few roundings of bin/inv and of hi) spare most
         // logits the rest.  In halves, as the bins: finite, up to `from`, which may be -infinity.
         float from = lo, to = hi;
-        if (normal) {
+        if (normal && bin >= 0) {
             const float width = range / kBins, off = 1e-6f * fabsf(half);
             if (bin < kBins - 1) from = fmaxf(lo, 2.0f * (half - (float)(bin + 1) * width * 1.00001f - off));
             to = fminf(hi, 2.0f * (half - (float)bin * width * 0.99999f + off));
@@ -280,7 +283,7 @@ __device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, f
             if (!some) return;
             unsigned in = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) in |= x[e] >= lo && x[e] <= hi && bin_of(x[e]) == bin ? 1u << e : 0;
+            for (int e = 0; e < 4; e++) in |= x[e] >= lo && x[e] <= hi && (bin < 0 || bin_of(x[e]) == bin) ? 1u << e : 0;
             for (int e = 0; e < 4; e++) {
                 if (!(in >> e & 1)) continue;
                 const float y = e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3];
@@ -304,6 +307,7 @@ __device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, f
         lo = from_ordered(s.lo);
         hi = from_ordered(s.hi);
         if (n <= kList) {
+            if (first) k.need = need_of(lane_value(sum_waves(wave_scan(t < n ? s.list_w[t] : 0), s, row.wave), 63));
             const int i = t % kList;
             if (i < n) {
                 const float x = s.list_x[i];
@@ -341,10 +345,10 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     __shared__ SampleLds s;
     __shared__ f4v copy[CAP ? CAP / 4 : 1];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = blockIdx.x;
-    const float *logits = a.logits + (long)r * a.ld;
+    const float *base = a.logits + (long)r * a.ld;
     Row<(CAP > 0)> row;
-    row.skip = (int)((uintptr_t)logits >> 2 & 3);
-    row.at = reinterpret_cast<const f4v *>(logits - row.skip);
+    row.skip = (int)((uintptr_t)base >> 2 & 3);
+    row.at = reinterpret_cast<const f4v *>(base - row.skip);
     row.wave = wave;
     row.vocab = a.vocab;
     row.turns = (a.vocab + row.skip + 4 * kThreads - 1) / (4 * kThreads);
@@ -398,30 +402,31 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
     // stays: logits above `last`, and the first `ties` of its `equals`
     float last = floor_;
     u64 ties = (u64)a.vocab, equals = 0;
+    int logits = a.vocab;            // from `last` on, or more
     if (top_k > 0 && top_k < a.vocab) {
-        const Mark k = find_mark(row, s, floor_, top, true, CountOf(), [&](u64 weigh) { return min((u64)top_k, weigh); });
+        const Mark k = find_mark(row, s, floor_, top, a.vocab, CountOf(), [&](u64 weigh) { return min((u64)top_k, weigh); });
         last = k.value;
         equals = k.equals;
         ties = k.need - k.before;
+        logits = (int)(k.before + k.equals);
     }
     if (!(top_p >= 1.0f)) {
         const u64 dropped = equals > ties ? (equals - ties) * weight(last) : 0;
         // stays: sums before it under top_p * total, so the last is where the sum reaches it
-        const Mark k = find_mark(row, s, last, top, equals == 0 || top_k > a.vocab / 32, weight, [&](u64 sum) {
+        const Mark k = find_mark(row, s, last, top, logits, weight, [&](u64 sum) {
             const double lim = top_p > 0.0f ? (double)top_p * (double)(sum - dropped) : 0.0;
             u64 need = (u64)lim;
             if ((double)need < lim) need++;
             return max(need, (u64)1);
         });
-        const u64 each = weight(k.value), n = (k.need - k.before + each - 1) / each;
-        if (k.value > last) {
-            last = k.value;
-            equals = k.equals / each;
-            ties = n;
-        } else {
-            equals = k.equals / each;
-            ties = min(ties, n);
-        }
+        // how many equals it has, and how many of them until the mark (of numbers under 2^18 a quotient is near enough)
+        const u64 each = weight(k.value), rest = k.need - k.before;
+        const double one = 1.0 / (double)each;
+        u64 n = (u64)((double)rest * one);
+        n += n * each < rest ? 1 : 0;                        // (rest/each a little under a whole number: one more than its floor)
+        equals = (u64)((double)k.equals * one + 0.5);
+        ties = k.value > last ? n : min(ties, n);
+        last = k.value;
     }
     // more equals of the last than stay: the index of the last that does
     int cut = INT_MAX;
@@ -453,6 +458,7 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
         // (a wave's accesses to shared memory are in order)
         int n = 0;                                           // in the wave's queue, under 64 between turns of the loop
         row.each([&](const f4v &v, int q) {
+            if (!__any(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= last)) return;
             bool in[4];
             u64 mask[4];
 #pragma unroll
@@ -460,7 +466,6 @@ __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_s
                 in[e] = stays(v[e], row.index(q) + e);
                 mask[e] = __ballot(in[e]);
             }
-            if (!(mask[0] | mask[1] | mask[2] | mask[3])) return;
             if (!~(mask[0] & mask[1] & mask[2] & mask[3])) { // none to pick out
 #pragma unroll
                 for (int e = 0; e < 4; e++) w += weight(v[e]);
