@@ -212,7 +212,7 @@ struct Mark { float value; u64 before, equals, need; };
 
 template <bool LOCAL, typename M, typename F>
 __device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, float lo, float hi, int logits, const M &measure, F &&need_of) {
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, lane = t & 63;
     Mark k = {hi, 0, 0, 0};
     bool first = true;
     for (int step = 0; step < 64; step++) {                  // (each takes 11 bits of the bounds' distance: under 40)
@@ -267,52 +267,53 @@ __device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, f
         } else {
             __syncthreads();
         }
-        // Bounds a little outside of the bin's (its border is off by a few roundings of bin/inv and of hi) spare most
-        // logits the rest.  In halves, as the bins: finite, up to `from`, which may be -infinity.
+        // Bounds a little outside of the bin's (its border is off by a few roundings of bin/inv and of hi, and half
+        // of a subnormal hi by one of its own) spare most logits the rest.  In halves, as the bins: finite, up to `from`, which may be -infinity.
         float from = lo, to = hi;
         if (normal && bin >= 0) {
-            const float width = range / kBins, off = 1e-6f * fabsf(half);
+            const float width = range / kBins, off = 1e-6f * fabsf(half) + 1e-37f;
             if (bin < kBins - 1) from = fmaxf(lo, 2.0f * (half - (float)(bin + 1) * width * 1.00001f - off));
             to = fminf(hi, 2.0f * (half - (float)bin * width * 0.99999f + off));
         }
         float least = INFINITY, most = -INFINITY;
         row.each([&](const f4v &x, int) {
-            bool some = false;
+            bool in[4], some = false;
 #pragma unroll
-            for (int e = 0; e < 4; e++) some |= x[e] >= from && x[e] <= to;
-            if (!some) return;
-            unsigned in = 0;
+            for (int e = 0; e < 4; e++) some |= in[e] = x[e] >= from && x[e] <= to;
+            if (!__any(some)) return;
+            u64 mask[4];
+            int n = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) in |= x[e] >= lo && x[e] <= hi && (bin < 0 || bin_of(x[e]) == bin) ? 1u << e : 0;
             for (int e = 0; e < 4; e++) {
-                if (!(in >> e & 1)) continue;
-                const float y = e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3];
-                least = fminf(least, y);
-                most = fmaxf(most, y);
-                // (the count stops a little above kList)
-                if (*(volatile int *)&s.members <= kList) {
-                    const int at = atomicAdd(&s.members, 1);
-                    if (at < kList) { s.list_x[at] = y; s.list_w[at] = measure(y); }
-                }
+                in[e] &= x[e] >= lo && x[e] <= hi && (bin < 0 || bin_of(x[e]) == bin);
+                mask[e] = __ballot(in[e]);
+                n += __popcll(mask[e]);
+                least = fminf(least, in[e] ? x[e] : INFINITY);
+                most = fmaxf(most, in[e] ? x[e] : -INFINITY);
+            }
+            if (n == 0) return;
+            int at = lane == 0 ? atomicAdd(&s.members, n) : 0;
+            at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int mine = (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask[e] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask[e], at));
+                if (in[e] && mine < kList) s.list_x[mine] = x[e];
+                at += __popcll(mask[e]);
             }
         });
-        least = -group_max<64>(-least);
-        most = group_max<64>(most);
-        if ((t & 63) == 0 && least <= most) {
-            atomicMin(&s.lo, ordered(least));
-            atomicMax(&s.hi, ordered(most));
-        }
         __syncthreads();
         const int n = s.members;
-        lo = from_ordered(s.lo);
-        hi = from_ordered(s.hi);
         if (n <= kList) {
-            if (first) k.need = need_of(lane_value(sum_waves(wave_scan(t < n ? s.list_w[t] : 0), s, row.wave), 63));
-            const int i = t % kList;
+            // All pairs of them, each member's by as many threads as there are.
+            const u64 own = t < n ? measure(s.list_x[t]) : 0;
+            if (t < n) s.list_w[t] = own;
+            const u64 sums = sum_waves(wave_scan(own), s, row.wave);
+            if (first) k.need = need_of(lane_value(sums, 63));
+            const int width = n <= 64 ? 64 : kList, i = t % width;
             if (i < n) {
                 const float x = s.list_x[i];
                 u64 above = 0, equal = 0;
-                for (int j = t / kList; j < n; j += kThreads / kList) {
+                for (int j = t / width; j < n; j += kThreads / width) {
                     const float y = s.list_x[j];
                     const u64 w = s.list_w[j];
                     above += y > x ? w : 0;
@@ -332,6 +333,15 @@ __device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, f
             k.equals = s.sum;
             return k;
         }
+        least = -group_max<64>(-least);
+        most = group_max<64>(most);
+        if (lane == 0 && least <= most) {
+            atomicMin(&s.lo, ordered(least));
+            atomicMax(&s.hi, ordered(most));
+        }
+        __syncthreads();
+        lo = from_ordered(s.lo);
+        hi = from_ordered(s.hi);
         __syncthreads();
     }
     return k;
