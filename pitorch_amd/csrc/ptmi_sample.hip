@@ -15,12 +15,12 @@
 // Weights are whole multiples of 2^-44 in 64 bits: sums of them are exact and
 // the same in any order, so the atomics of the bins leave the result as it is.
 //
-// A row is one compute unit's work, and its vector instructions bound it: one
-// per logit is 16 cycles of 1024 logits.  Of the 70 thousand cycles of a row of
-// 32000 under top_p alone, the pass that fills the bins (a weight each) takes
-// 24, the one that takes members out 10, the draw 18, the load 10.  That row:
-// 31 us; 64 rows of it with all sets of filters: 41; 509 rows of 50259, two
-// rows on a unit: 130 us (simple form, a bisection over the row: 177, 223, 535).
+// A row is one compute unit's work.  Of the 49 thousand cycles of a row of
+// 32000 under top_p alone, the load takes 4, the pass that fills the bins (a
+// weight each, some 35 instructions) 19, the search behind it 9, the draw 12;
+// the count under top_k 10, as the bins' atomics go.  That row: 20.4 us; 64 rows
+// of it with all sets of filters: 29.5; 509 rows of 50259, two rows on a unit:
+// 90 (simple form, a bisection over the row: 177, 223, 535).
 #include "ptmi_paged.h"
 
 #include <cfloat>
@@ -267,8 +267,9 @@ __device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, f
         } else {
             __syncthreads();
         }
-        // Bounds a little outside of the bin's (its border is off by a few roundings of bin/inv and of hi, and half
-        // of a subnormal hi by one of its own) spare most logits the rest.  In halves, as the bins: finite, up to `from`, which may be -infinity.
+        // Bounds a little outside of the bin's (its border is off by a few roundings of bin/inv and of hi, and half of
+        // a subnormal hi by one of its own) spare most logits the rest.  In halves, as the bins: finite, up to `from`,
+        // which may be -infinity.
         float from = lo, to = hi;
         if (normal && bin >= 0) {
             const float width = range / kBins, off = 1e-6f * fabsf(half) + 1e-37f;
@@ -349,7 +350,7 @@ __device__ __forceinline__ Mark find_mark(const Row<LOCAL> &row, SampleLds &s, f
 
 // CAP: logits that the copy in shared memory holds; 0: no copy.  Where two
 // rows fit a compute unit's shared memory the registers are held to it, some
-// spilled: 509 rows of 50259 take 139 us so, 162 at one row a unit.
+// spilled: 509 rows of 50259 took 139 us so, 162 at one row a unit.
 template <int CAP>
 __global__ __launch_bounds__(kThreads, CAP == 0 || CAP == 8192 ? 8 : 4) void k_sample(SampleArgs a) {
     __shared__ SampleLds s;
