@@ -6,10 +6,11 @@
 //   m' = max(m, s), l' = l 2^(m - m') + sum 2^(s - m'), o' = o 2^(m - m') + sum 2^(s - m') v
 // with scores s = (scale log2(e) q).k, so that every e^x is one 2^x.
 //
-// Three kernels, by M.  Up to 16 rows (single tokens, a few tokens) are bound
+// Four kernels, by M and the type of the pages.  Up to 16 rows (single tokens, a few tokens) are bound
 // by the bytes of the cache: k_attn_stream for up to 4, on the vector units,
-// k_attn_few through the fp32 matrix instructions.  More rows are bound by the
-// products: k_attn_tile, on the 16-bit matrix cores.  Against the simple form
+// k_attn_few through the fp32 matrix instructions, k_attn_few_b16 through the
+// bf16 ones.  More rows are bound by the products: k_attn_tile, on the 16-bit
+// matrix cores.  Against the simple form
 // (a wave a row, a key at a time): 64 requests of one token and 12 heads of 64,
 // 617 -> 40 us; 2 of 70 to 131 thousand positions, 32 heads on 8 of 128 in
 // bf16, 115600 -> 180; 16 chunks of 512 tokens, 12 heads of 64, 23100 -> 330.
@@ -321,14 +322,14 @@ __device__ __forceinline__ f4v mfma4(float a, float b, f4v c) {
 constexpr int few_pitch(int dt) { return dt > 2 ? 128 : 64; }
 constexpr int few_part(int dt) { return kFewRows * few_pitch(dt) + 2 * kFewRows; }
 
-template <int HQ, bool PAD, bool BF16>
+template <int HQ, bool BF16>
 struct FewBlock {                    // 16 keys of one head
     Raw4<BF16> k[HQ], v[4][HQ > 4 ? 2 : 1];
     long off;                        // lane's key li; -1: not there
 };
 
 template <int HQ, bool PAD, bool BF16>
-__device__ __forceinline__ void few_load(const AttnArgs &a, FewBlock<HQ, PAD, BF16> &b, int n4) {
+__device__ __forceinline__ void few_load(const AttnArgs &a, FewBlock<HQ, BF16> &b, int n4) {
     constexpr int C4 = HQ > 4 ? 2 : 1;
     const int lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -349,12 +350,70 @@ __device__ __forceinline__ void few_load(const AttnArgs &a, FewBlock<HQ, PAD, BF
     }
 }
 
-template <int HQ, bool PAD, bool BF16>
+struct FewLds {
+    static constexpr int NW = kThreads / 64;
+    float m[NW][kFewRows], l[NW][kFewRows];
+};
+
+// Joins the four waves' (m, l, acc) of a key head's stretch [u, ue): to the output, or to the workgroup's part.
+template <int HQ>
+__device__ __forceinline__ void few_out(const AttnArgs &a, const Item &it, int wg, long u, long ue, const f4v (&acc)[HQ > 4 ? 8 : 4],
+                                        float m, float l, int hd, float *red, FewLds &st) {
+    constexpr int C4 = HQ > 4 ? 2 : 1, FP = few_pitch(HQ / 2), PITCH = FP + 4, NW = FewLds::NW;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+    const int n4 = hd >> 2, G = a.group.d, M = it.r.n * G;
+    // the four waves' sums, one maximum for all
+    l = xsum32(xsum16(l));
+    if (g == 0) { st.m[wave][li] = m; st.l[wave][li] = l; }
+    __syncthreads();
+    float gm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; w++) gm = fmaxf(gm, st.m[w][li]);
+    const float ref = gm == -INFINITY ? 0.0f : gm, f = exp2_hw(m - ref);
+    if (li < M) {
+#pragma unroll
+        for (int c = 0; c < C4; c++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const f4v o = {acc[4 * c][r], acc[4 * c + 1][r], acc[4 * c + 2][r], acc[4 * c + 3][r]};
+                *reinterpret_cast<f4v *>(red + (wave * kFewRows + li) * PITCH + 4 * (16 * c + 4 * g + r)) = o * f;
+            }
+    }
+    __syncthreads();
+    const bool whole = u == it.a && ue == it.b;
+    float *part = a.parts + (long)(2 * wg + (u == it.a)) * few_part(HQ / 2);
+    for (int e = threadIdx.x; e < M * n4; e += kThreads) {
+        const int i = e / n4, c = e - i * n4;
+        f4v o = *reinterpret_cast<const f4v *>(red + i * PITCH + 4 * c);
+#pragma unroll
+        for (int w = 1; w < NW; w++) o += *reinterpret_cast<const f4v *>(red + (w * kFewRows + i) * PITCH + 4 * c);
+        float im = -INFINITY, il = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; w++) im = fmaxf(im, st.m[w][i]);
+        const float iref = im == -INFINITY ? 0.0f : im;
+#pragma unroll
+        for (int w = 0; w < NW; w++) il += st.l[w][i] * exp2_hw(st.m[w][i] - iref);
+        if (whole) {
+            const int t = a.group.quot(i), r = it.r.row0 + t;
+            if ((unsigned)r < (unsigned)a.rows)
+                *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(it.kvh * G + i - t * G) * hd + 4 * c) =
+                    o * (il == 0.0f ? 0.0f : 1.0f / il);
+        } else {
+            *reinterpret_cast<f4v *>(part + i * FP + 4 * c) = o;
+            if (c == 0) {
+                part[kFewRows * FP + 2 * i] = im;
+                part[kFewRows * FP + 2 * i + 1] = il;
+            }
+        }
+    }
+}
+
+template <int HQ, bool PAD>
 __global__ __launch_bounds__(kThreads, 2) void k_attn_few(AttnArgs a) {
-    constexpr int C4 = HQ > 4 ? 2 : 1, NC = 4 * C4, FP = few_pitch(HQ / 2), PITCH = FP + 4, NW = kThreads / 64;
+    constexpr int C4 = HQ > 4 ? 2 : 1, NC = 4 * C4, NW = kThreads / 64;
     __shared__ Axis axis;
-    __shared__ __align__(16) float red[NW * kFewRows * PITCH];
-    __shared__ float st_m[NW][kFewRows], st_l[NW][kFewRows];
+    __shared__ __align__(16) float red[NW * kFewRows * (few_pitch(HQ / 2) + 4)];
+    __shared__ FewLds st;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
     const int hd = PAD ? a.hd : 16 * HQ, n4 = hd >> 2, G = a.group.d;
     const Split split(axis_init<false>(a, axis), gridDim.x);
@@ -385,13 +444,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_few(AttnArgs a) {
         // this wave's 16 keys of every unit; two blocks of keys and one more of page numbers in flight
         int kb = (int)(u - it.a) * 4 + wave;
         const int kend = (int)(ue - it.a) * 4;
-        FewBlock<HQ, PAD, BF16> cur, nxt;
+        FewBlock<HQ, false> cur, nxt;
         cur.off = key_offset(a, kb * 16 + li, len, page_of(a, it.s, kb * 16 + li, len), it.kvh);
         int pg = page_of(a, it.s, (kb + NW) * 16 + li, len);
-        few_load(a, cur, n4);
+        few_load<HQ, PAD>(a, cur, n4);
         for (; kb < kend; kb += NW) {
             nxt.off = kb + NW < kend ? key_offset(a, (kb + NW) * 16 + li, len, pg, it.kvh) : -1;
-            few_load(a, nxt, n4);
+            few_load<HQ, PAD>(a, nxt, n4);
             pg = page_of(a, it.s, (kb + 2 * NW) * 16 + li, len);
             f4v s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
@@ -461,50 +520,221 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_few(AttnArgs a) {
                 for (int c = 0; c < NC; c++) acc[c] = mfma4(v[t][c >> 2][c & 3], p[t], acc[c]);
             cur = nxt;
         }
-        // the four waves' sums, one maximum for all
-        l = xsum32(xsum16(l));
-        if (g == 0) { st_m[wave][li] = m; st_l[wave][li] = l; }
+        few_out<HQ>(a, it, wg, u, ue, acc, m, l, hd, red, st);
+        if (ue == u1) note_cut(a, wg, split, it, u, ue);
         __syncthreads();
-        float gm = -INFINITY;
+        u = ue;
+    }
+}
+
+// bf16 pages: v_mfma_f32_16x16x32_bf16, whose operands are eight elements of a
+// lane, takes keys and values as they are.  A query or weight is three of
+// them, its leading 8 bits, the next 8 and the rest (cut off, not rounded:
+// nothing overflows, and the three are all 24), so a product is as exact as in
+// fp32.  Two blocks of 16 keys are one contraction: slot 4 x + s of lane group
+// g is key 4g + s of block x, so P^T stands as S^T left it and lane li's
+// values of eight keys are picked apart into V^T's rows.
+// The fp32 instructions would bound bf16 pages: 64 requests of one token at
+// 8192, 32 heads on 4 of 128, took 277 us, now 218 (1.07 GB, 4.9 TB/s); 20 on 4
+// of 80, 248 -> 165; 8 new tokens of 12 heads of 64 at 4096, 213 -> 176.  The
+// queries' thirds in registers spill what is on its way: 352 us for the first.
+// Three workgroups a unit where heads are small: 113 us for the third with
+// heads of 32, 175 with two.
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef unsigned u4v __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f4v mfma_b16(u4v a, u4v b, f4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+}
+// The upper (lower) halves of a and b side by side, a's first.
+__device__ __forceinline__ unsigned upper_halves(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
+__device__ __forceinline__ unsigned lower_halves(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
+
+struct Thirds {                      // of eight floats
+    u4v h, m, l;
+    __device__ __forceinline__ void set(int i, float x, float y) {   // elements 2 i and 2 i + 1
+        const unsigned xb = __float_as_uint(x), yb = __float_as_uint(y);
+        h[i] = upper_halves(xb, yb);
+        const float x1 = x - __uint_as_float(xb & 0xFFFF0000u), y1 = y - __uint_as_float(yb & 0xFFFF0000u);
+        const unsigned x1b = __float_as_uint(x1), y1b = __float_as_uint(y1);
+        m[i] = upper_halves(x1b, y1b);
+        l[i] = upper_halves(__float_as_uint(x1 - __uint_as_float(x1b & 0xFFFF0000u)),
+                            __float_as_uint(y1 - __uint_as_float(y1b & 0xFFFF0000u)));
+    }
+};
+
+template <int HQ, bool PAD>
+__global__ __launch_bounds__(kThreads, HQ <= 4 ? 3 : 2) void k_attn_few_b16(AttnArgs a) {
+    constexpr int C4 = HQ > 4 ? 2 : 1, NC = 4 * C4, NW = kThreads / 64;
+    __shared__ Axis axis;
+    __shared__ __align__(16) float red[NW * kFewRows * (few_pitch(HQ / 2) + 4)];
+    __shared__ FewLds st;
+    __shared__ u4v qs[HQ / 2][3][64];                        // the queries' thirds (registers hold keys and values on their way)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
+    const int hd = PAD ? a.hd : 16 * HQ, n4 = hd >> 2, G = a.group.d;
+    const Split split(axis_init<false>(a, axis), gridDim.x);
+    const int wg = stretch_of_block();
+    const long u1 = split.first(wg + 1);
+    if (threadIdx.x == 0 && split.first(wg) == u1) a.cuts[wg].parts = 0;
+    for (long u = split.first(wg); u < u1;) {
+        const Item it = axis_item<false>(a, axis, u);
+        const long ue = min(u1, it.b);
+        const int M = it.r.n * G, len = it.r.len;
+        const int tok = a.group.quot(li), row = it.r.row0 + tok;             // this lane's row
+        const bool live = li < M && (unsigned)row < (unsigned)a.rows;
+        const float *qrow = a.q + row * a.ldq + (long)(it.kvh * G + li - tok * G) * hd;
+        f4v qx[HQ];
+        float top = 0.0f;
 #pragma unroll
-        for (int w = 0; w < NW; w++) gm = fmaxf(gm, st_m[w][li]);
-        const float ref = gm == -INFINITY ? 0.0f : gm, f = exp2_hw(m - ref);
-        if (li < M) {
+        for (int j = 0; j < HQ; j++) {
+            const int i = 4 * j + g;
+            qx[j] = f4v{0.f, 0.f, 0.f, 0.f};
+            if (live && (!PAD || i < n4)) qx[j] = *reinterpret_cast<const f4v *>(qrow + 4 * i) * a.qscale;
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(qx[j][e]));
+        }
+        LanePair pr = pl16(top);
+        pr = pl32(fmaxf(pr.lo, pr.hi));
+        // a third under 2^-126 would lose bits: rows that are all small count in 2^-64
+        const bool small = fmaxf(pr.lo, pr.hi) < 0x1p-80f;
+        const float up = small ? 0x1p64f : 1.0f, down = small ? 0x1p-64f : 1.0f;
+        static_assert(HQ / 2 <= NW, "a wave's share of the row: elements of float4s 8 j + g and 8 j + 4 + g");
+#pragma unroll
+        for (int j = 0; j < HQ / 2; j++) {
+            if (j != wave) continue;
+            Thirds q;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const f4v x = qx[2 * j + s] * up;
+                q.set(2 * s, x.x, x.y);
+                q.set(2 * s + 1, x.z, x.w);
+            }
+            qs[j][0][lane] = q.h;
+            qs[j][1][lane] = q.m;
+            qs[j][2][lane] = q.l;
+        }
+        __syncthreads();
+        const int see = len - it.r.n + tok + 1;             // keys [0, see)
+        const int see0 = len - it.r.n + 1;                  // of the first row
+        f4v acc[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) acc[c] = f4v{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.0f;
+        // this wave's 16 keys of two units at a time; two pairs of blocks and one more of page numbers in flight
+        int kb = (int)(u - it.a) * 4 + wave;
+        const int kend = (int)(ue - it.a) * 4;
+        auto key_of = [&](int b) { return b * 16 + li; };
+        auto page_at = [&](int b) { return b < kend ? page_of(a, it.s, key_of(b), len) : -1; };
+        FewBlock<HQ, true> cur[2], nxt[2];
+        int pg[2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            cur[x].off = key_offset(a, key_of(kb + x * NW), len, page_at(kb + x * NW), it.kvh);
+            pg[x] = page_at(kb + (2 + x) * NW);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; x++) few_load<HQ, PAD>(a, cur[x], n4);
+        for (; kb < kend; kb += 2 * NW) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                nxt[x].off = key_offset(a, key_of(kb + (2 + x) * NW), len, pg[x], it.kvh);
+                few_load<HQ, PAD>(a, nxt[x], n4);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++) pg[x] = page_at(kb + (4 + x) * NW);
+            asm volatile("" ::: "memory");                   // (queries are read again, not kept)
+            f4v s[2];
+            bool use[2][4];
+            float bm = -INFINITY;
+            s[0] = s[1] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < HQ / 2; j++) {
+                const u4v qh = qs[j][0][lane], qm = qs[j][1][lane], ql = qs[j][2][lane];
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const u4v k = {cur[x].k[2 * j].x.x, cur[x].k[2 * j].x.y, cur[x].k[2 * j + 1].x.x, cur[x].k[2 * j + 1].x.y};
+                    s[x] = mfma_b16(k, ql, s[x]);
+                    s[x] = mfma_b16(k, qm, s[x]);
+                    s[x] = mfma_b16(k, qh, s[x]);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                s[x] *= down;
+                const unsigned there = (unsigned)(__ballot(cur[x].off >= 0) >> (4 * g));   // bit r: key 4g + r
+                const int key = (kb + x * NW) * 16 + 4 * g;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    use[x][r] = (there >> r & 1) && key + r < see;
+                    bm = use[x][r] ? fmaxf(bm, s[x][r]) : bm;
+                }
+            }
+            pr = pl16(bm);
+            bm = fmaxf(pr.lo, pr.hi);
+            pr = pl32(bm);
+            const float mn = fmaxf(m, fmaxf(pr.lo, pr.hi)), ref = mn == -INFINITY ? 0.0f : mn;
+            if (__any(mn > m)) {
+                const float f = exp2_hw(m - ref);
+                l *= f;
+                m = mn;
+#pragma unroll
+                for (int c = 0; c < NC; c++) acc[c] *= f;
+            }
+            Thirds p;
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const float e0 = exp2_hw(s[x][r] - ref), e1 = exp2_hw(s[x][r + 1] - ref);
+                    const float p0 = use[x][r] ? e0 : 0.0f, p1 = use[x][r + 1] ? e1 : 0.0f;
+                    l += p0;
+                    l += p1;
+                    p.set(2 * x + r / 2, p0, p1);
+                }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int k0 = (kb + x * NW) * 16;
+                if (k0 + 16 <= see0) continue;
+                // rows that do not see a key must not meet its value if that is not finite (0 * NaN):
+                // it leaves the product, and the rows that see it get a NaN in its place
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int c = 0; c < C4; c++) {
+                        const f4v v = widen(cur[x].v[t][c]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const unsigned long bad = __ballot(!finite_bits(v[e]));
+                            if (!bad) continue;
+#pragma unroll
+                            for (int h = 0; h < 4; h++)
+#pragma unroll
+                                for (int r = 0; r < 4; r++)
+                                    if ((bad >> (16 * h + 4 * g + r) & 1) && k0 + 4 * h + t < see) acc[4 * c + e][r] = NAN;
+                        }
+                        drop_odd(cur[x].v[t][c]);
+                    }
+            }
 #pragma unroll
             for (int c = 0; c < C4; c++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const f4v o = {acc[4 * c][r], acc[4 * c + 1][r], acc[4 * c + 2][r], acc[4 * c + 3][r]};
-                    *reinterpret_cast<f4v *>(red + (wave * kFewRows + li) * PITCH + 4 * (16 * c + 4 * g + r)) = o * f;
+                for (int e = 0; e < 4; e++) {
+                    u4v v;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint2 y = cur[i >> 1].v[2 * (i & 1)][c].x, z = cur[i >> 1].v[2 * (i & 1) + 1][c].x;
+                        v[i] = e & 1 ? upper_halves(e & 2 ? y.y : y.x, e & 2 ? z.y : z.x)
+                                     : lower_halves(e & 2 ? y.y : y.x, e & 2 ? z.y : z.x);
+                    }
+                    f4v &o = acc[4 * c + e];
+                    o = mfma_b16(v, p.l, o);
+                    o = mfma_b16(v, p.m, o);
+                    o = mfma_b16(v, p.h, o);
                 }
+#pragma unroll
+            for (int x = 0; x < 2; x++) cur[x] = nxt[x];
         }
-        __syncthreads();
-        const bool whole = u == it.a && ue == it.b;
-        float *part = a.parts + (long)(2 * wg + (u == it.a)) * few_part(HQ / 2);
-        for (int e = threadIdx.x; e < M * n4; e += kThreads) {
-            const int i = e / n4, c = e - i * n4;
-            f4v o = *reinterpret_cast<const f4v *>(red + i * PITCH + 4 * c);
-#pragma unroll
-            for (int w = 1; w < NW; w++) o += *reinterpret_cast<const f4v *>(red + (w * kFewRows + i) * PITCH + 4 * c);
-            float im = -INFINITY, il = 0.0f;
-#pragma unroll
-            for (int w = 0; w < NW; w++) im = fmaxf(im, st_m[w][i]);
-            const float iref = im == -INFINITY ? 0.0f : im;
-#pragma unroll
-            for (int w = 0; w < NW; w++) il += st_l[w][i] * exp2_hw(st_m[w][i] - iref);
-            if (whole) {
-                const int t = a.group.quot(i), r = it.r.row0 + t;
-                if ((unsigned)r < (unsigned)a.rows)
-                    *reinterpret_cast<f4v *>(a.out + r * a.ldo + (long)(it.kvh * G + i - t * G) * hd + 4 * c) =
-                        o * (il == 0.0f ? 0.0f : 1.0f / il);
-            } else {
-                *reinterpret_cast<f4v *>(part + i * FP + 4 * c) = o;
-                if (c == 0) {
-                    part[kFewRows * FP + 2 * i] = im;
-                    part[kFewRows * FP + 2 * i + 1] = il;
-                }
-            }
-        }
+        few_out<HQ>(a, it, wg, u, ue, acc, m, l, hd, red, st);
         if (ue == u1) note_cut(a, wg, split, it, u, ue);
         __syncthreads();
         u = ue;
@@ -837,6 +1067,8 @@ __device__ __forceinline__ unsigned finite_top(unsigned top, const f4v &x) {
     return top;
 }
 
+// Waves of a tile of heads up to 32 dt: small ones leave room for two workgroups of four (12 heads of 64: 350 us, 370
+// with one of eight); for large ones keys are split for twice the rows (32 heads on 8 of 128, bf16: 417 us, 617 with four).
 constexpr int tile_waves(int dt) { return dt <= 2 ? 4 : 8; }
 constexpr int tile_part(int dt) { return 32 * tile_waves(dt) * (32 * dt + 2); }   // floats
 
@@ -1326,8 +1558,9 @@ __global__ __launch_bounds__(kThreads) void k_attn_join(AttnArgs a, int n_few, c
 
 // ── launch ───────────────────────────────────────────────────────────────
 // Workgroups: what the chip holds at once.  More would split heads further
-// and start anew (64 requests of 32 heads on 4, 1024 bf16 positions of 128:
-// 104 us on 1024 workgroups, 54 on the 512 that fit), fewer leave it idle
+// and start anew (64 requests of 32 heads on 4, 1024 bf16 positions of 128,
+// through the fp32 instructions: 104 us on 1024 workgroups, 54 on the 512 that
+// fit), fewer leave it idle
 // (1024 requests of 12 heads, 100 positions of 64: 168 us on 512, 133 on 1024).
 constexpr int kFewGroups = 1024;                            // the most for few rows
 constexpr int kTileGroups = 512;
@@ -1340,8 +1573,8 @@ typedef void (*JoinFn)(AttnArgs, int, const Cut *, const float *);
 
 template <int HQ>
 Fn few_fn(int hd, bool b16) {
-    return hd == 16 * HQ ? (b16 ? k_attn_few<HQ, false, true> : k_attn_few<HQ, false, false>)
-                         : (b16 ? k_attn_few<HQ, true, true> : k_attn_few<HQ, true, false>);
+    return hd == 16 * HQ ? (b16 ? k_attn_few_b16<HQ, false> : k_attn_few<HQ, false>)
+                         : (b16 ? k_attn_few_b16<HQ, true> : k_attn_few<HQ, true>);
 }
 template <int MR, int C4>
 Fn stream_fn2(bool fast, bool b16) {

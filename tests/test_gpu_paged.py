@@ -370,7 +370,7 @@ def test_attention_scales(new, scale):
     assert_close(*run_attention([(150, new), (9, new)], 2, 2, 64, 16, pa.F32, seed=4, scale=scale))
 
 
-@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("new", [1, 8, 70])
 @pytest.mark.parametrize("kind", [pa.F32, pa.BF16])
 def test_attention_of_large_and_small_values(new, kind):
     """Keys and values of very different sizes from tile to tile and within a row."""
@@ -447,6 +447,29 @@ def test_attention_of_many_requests(news):
     reqs = [(int(rng.integers(0, 40)), int(rng.choice(news))) for _ in range(600)]
     assert_close(*run_attention(reqs, 2, 1, 32, 8, pa.F32, seed=12))
     assert_close(*run_attention(reqs, 1, 1, 16, 8, pa.BF16, seed=13, max_new=0))
+
+
+@pytest.mark.parametrize("heads,new", [(5, 1), (8, 1), (16, 1), (1, 5), (2, 7), (1, 16)])
+@pytest.mark.parametrize("hd", [4, 28, 64, 80, 96, 124, 128])
+def test_attention_of_five_to_sixteen_rows(hd, heads, new):
+    """Lengths around the pairs of 64 keys that such rows take at once, in both types of pages."""
+    lens = [0, 1, 47, 62, 63, 64, 65, 111, 126, 127, 128, 129, 191, 200, 640]
+    layout = ("tokens", "heads", "padded")[(hd + heads) % 3]
+    page = (16, 7, 24)[new % 3]
+    for kind in (pa.BF16, pa.F32):
+        assert_close(*run_attention([(n, new) for n in lens], 2 * heads, 2, hd, page, kind, layout, seed=hd + new))
+
+
+@pytest.mark.parametrize("new", [1, 2, 8, 70])
+@pytest.mark.parametrize("kind", [pa.F32, pa.BF16])
+@pytest.mark.parametrize("size", [1e-37, 1e-20, 1e37])
+def test_attention_of_keys_and_queries_of_any_size(new, kind, size):
+    """Queries that make up for the size of the keys; values at both ends of the type."""
+    def edit(d):
+        d["k"] *= np.float32(size)
+        d["q"] *= np.float32(1 / size)
+        d["v"] *= np.float32(1e36)
+    assert_close(*run_attention([(100, new), (9, new)], 2, 2, 64, 16, kind, seed=21, edit=edit, stale=0.0))
 
 
 @pytest.mark.parametrize("new", [1, 2, 40])
