@@ -494,7 +494,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_few(AttnArgs a) {
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int c = 0; c < C4; c++) v[t][c] = widen(cur.v[t][c]);
-            if (kb * 16 + 16 > see0) {
+            if (max(kb * 16, see0) < min(kb * 16 + 16, len)) {
                 // rows that do not see a key must not meet its value if that is not finite (0 * NaN):
                 // it leaves the product, and the rows that see it get a NaN in its place
 #pragma unroll
@@ -535,11 +535,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_attn_few(AttnArgs a) {
 // g is key 4g + s of block x, so P^T stands as S^T left it and lane li's
 // values of eight keys are picked apart into V^T's rows.
 // The fp32 instructions would bound bf16 pages: 64 requests of one token at
-// 8192, 32 heads on 4 of 128, took 277 us, now 218 (1.07 GB, 4.9 TB/s); 20 on 4
-// of 80, 248 -> 165; 8 new tokens of 12 heads of 64 at 4096, 213 -> 176.  The
-// queries' thirds in registers spill what is on its way: 352 us for the first.
-// Three workgroups a unit where heads are small: 113 us for the third with
-// heads of 32, 175 with two.
+// 8192, 32 heads on 4 of 128, took 277 us, now 220 (1.07 GB, 4.9 TB/s); 20 on 4
+// of 80, 248 -> 170; 8 new tokens of 12 heads of 64 at 4096, 213 -> 180.  (One
+// request at 100: 12.7 -> 13.8, for the thirds.)  The queries' thirds in
+// registers spill what is on its way: 352 us for the first.  Three workgroups a
+// unit where heads are small: 123 us for the last with heads of 32, 175 with two.
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 typedef unsigned u4v __attribute__((ext_vector_type(4)));
 
@@ -583,6 +583,20 @@ __global__ __launch_bounds__(kThreads, HQ <= 4 ? 3 : 2) void k_attn_few_b16(Attn
         const int tok = a.group.quot(li), row = it.r.row0 + tok;             // this lane's row
         const bool live = li < M && (unsigned)row < (unsigned)a.rows;
         const float *qrow = a.q + row * a.ldq + (long)(it.kvh * G + li - tok * G) * hd;
+        // this wave's 16 keys of two units at a time; two pairs of blocks and one more of page numbers in flight
+        int kb = (int)(u - it.a) * 4 + wave;
+        const int kend = (int)(ue - it.a) * 4;
+        auto key_of = [&](int b) { return b * 16 + li; };
+        auto page_at = [&](int b) { return b < kend ? page_of(a, it.s, key_of(b), len) : -1; };
+        FewBlock<HQ, true> cur[2], nxt[2];
+        int pg[2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            cur[x].off = key_offset(a, key_of(kb + x * NW), len, page_at(kb + x * NW), it.kvh);
+            pg[x] = page_at(kb + (2 + x) * NW);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; x++) few_load<HQ, PAD>(a, cur[x], n4);
         f4v qx[HQ];
         float top = 0.0f;
 #pragma unroll
@@ -620,20 +634,6 @@ __global__ __launch_bounds__(kThreads, HQ <= 4 ? 3 : 2) void k_attn_few_b16(Attn
 #pragma unroll
         for (int c = 0; c < NC; c++) acc[c] = f4v{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.0f;
-        // this wave's 16 keys of two units at a time; two pairs of blocks and one more of page numbers in flight
-        int kb = (int)(u - it.a) * 4 + wave;
-        const int kend = (int)(ue - it.a) * 4;
-        auto key_of = [&](int b) { return b * 16 + li; };
-        auto page_at = [&](int b) { return b < kend ? page_of(a, it.s, key_of(b), len) : -1; };
-        FewBlock<HQ, true> cur[2], nxt[2];
-        int pg[2];
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            cur[x].off = key_offset(a, key_of(kb + x * NW), len, page_at(kb + x * NW), it.kvh);
-            pg[x] = page_at(kb + (2 + x) * NW);
-        }
-#pragma unroll
-        for (int x = 0; x < 2; x++) few_load<HQ, PAD>(a, cur[x], n4);
         for (; kb < kend; kb += 2 * NW) {
 #pragma unroll
             for (int x = 0; x < 2; x++) {
@@ -694,7 +694,7 @@ __global__ __launch_bounds__(kThreads, HQ <= 4 ? 3 : 2) void k_attn_few_b16(Attn
 #pragma unroll
             for (int x = 0; x < 2; x++) {
                 const int k0 = (kb + x * NW) * 16;
-                if (k0 + 16 <= see0) continue;
+                if (max(k0, see0) >= min(k0 + 16, len)) continue;
                 // rows that do not see a key must not meet its value if that is not finite (0 * NaN):
                 // it leaves the product, and the rows that see it get a NaN in its place
 #pragma unroll
