@@ -73,7 +73,7 @@ template <int CAP>
 __device__ PlanTotals plan_sums(const PlanArgs &a, PlanLds<CAP> &s, int count) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
     if (t == 0) s.bad = count < 0 || count > a.n_pages ? 8 : 0;
-    long take = 0, give = 0, rows = 0;                       // before this round's requests
+    long take = 0, give = 0, rows = 0;                       // before this turn's requests
     for (int i0 = 0; i0 < a.n; i0 += kPlanThreads) {
         const int i = i0 + t;
         int p = 0, f = 0;

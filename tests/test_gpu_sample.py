@@ -132,6 +132,23 @@ def test_logits_of_any_size(unit):
     compare(x, temperature=t, top_p=[0.3, 0.8, 0.5, 0.5, 0.9, 0.99], u=rng.random(6))
 
 
+@pytest.mark.parametrize("V", [1, 3, 255, 256, 257, 4100, 9000, 20001, 33000, 70001])
+@pytest.mark.parametrize("step", [0.0, 0.25])
+def test_how_many_stay(V, step):
+    """top_k around the numbers of logits that are compared at once or looked at one by one, with equals (step) and
+    without, and top_p behind it."""
+    rng = np.random.default_rng(V)
+    ks = [2, 17, 63, 64, 65, 255, 256, 257, 300, V // 32, V // 32 + 1, V - 1]
+    x = (rng.standard_normal((len(ks), V)) * 2).astype(np.float32)
+    if step:
+        x = (np.round(x / step) * step).astype(np.float32)
+    x[::3, : V // 2] = -np.inf
+    u, t = rng.random(len(ks)), np.full(len(ks), 0.9)
+    for p in (1.0, 0.97, 0.5):
+        compare(x, pad=1, temperature=t, top_k=ks, top_p=np.full(len(ks), p), u=u)
+    compare(x, temperature=t, top_k=ks, min_p=np.full(len(ks), 0.03), top_p=np.full(len(ks), 0.9), u=u)
+
+
 @pytest.mark.parametrize("V", [1000, 32000])
 def test_equal_logits(V):
     """Whole weights: every border is met exactly, and the first of equals counts."""
