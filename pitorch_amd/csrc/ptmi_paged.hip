@@ -16,15 +16,15 @@ namespace {
 // ended requests' pages went onto it, pool[i] below the old count and above
 // it the (i - count)-th given page, read where it comes from: so nothing that
 // is written here is read here.
-// A step's rows bound it: few fit one workgroup, which then also writes the
-// lengths; for many, workgroups that each hold all sums share the rows and
-// pages (k_paged_plan), and a launch behind them writes the lengths, which
-// may stand where the cached lengths were read (k_paged_plan_end).
+// A step's rows bound it: few fit one workgroup; for many, workgroups that
+// each hold all sums share the rows and pages.  The first one also writes the
+// lengths; only where these stand in the place of the cached lengths, which
+// other workgroups still read, does a launch of its own (k_paged_plan_end).
 // 16 requests of one token: 14.6 -> 4.9 us a call (sums of 1024 in 20 steps
 // with a barrier each before, now in two); 1021 requests, 44 thousand rows,
-// 14 thousand pages: 150 -> 12.4 us, 9 and 3.8 of them the two launches (one
-// workgroup, a request's pages and rows by one thread each before).  Both are
-// latency: a handful of dependent loads, and 0.4 MB written in the second.
+// 14 thousand pages: 150 -> 8.7 us, and 3.5 for the second launch where there is
+// one (one workgroup, a request's pages and rows by one thread each before).
+// Both are latency: a handful of dependent loads, and 0.4 MB written.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSmall = 1024, kPlanMost = 8192;          // requests whose sums fit in shared memory
 constexpr int kPlanOneRows = 4096;                          // rows that one workgroup writes
@@ -42,7 +42,7 @@ struct PlanArgs {
     int *kv_len, *pool_left, *row_start, *row_pos, *row_slot;
     int max_rows;
     int *status;
-    bool one;                        // one workgroup does it all
+    bool end;                        // the first workgroup writes the lengths as well
 };
 
 // Sums over the requests before i; entry n: of all.
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(PlanArgs a) {
         }
     }
     for (int r = (all.refused ? 0 : (int)all.rows) + first; r < a.max_rows; r += step) a.row_pos[r] = a.row_slot[r] = -1;
-    if (a.one) plan_end(a, s, all, count);
+    if (a.end && blockIdx.x == 0) plan_end(a, s, all, count);
 }
 
 template <int CAP>
@@ -296,14 +296,15 @@ int ptmi_paged_plan_dev(const int *past, const int *fresh, int n_requests, int *
     if (st) return st;
     DeviceScope dev;
     if ((st = dev.enter())) return st;
+    const bool one = max_rows <= kPlanOneRows;
     const PlanArgs a = {past, fresh, n_requests, pool, pool_count, n_pages, FastDiv(page_size), block_table,
                         table_width, kv_len, pool_left, row_start, row_pos, row_slot, max_rows, status,
-                        max_rows <= kPlanOneRows};
+                        one || (kv_len != past && pool_left != pool_count)};
     hipStream_t s = stream ? (hipStream_t)stream : lib_stream();
     const bool small = n_requests <= kPlanSmall;
-    const int groups = a.one ? 1 : std::min(256, (max_rows + kPlanThreads - 1) / kPlanThreads);
+    const int groups = one ? 1 : std::min(256, (max_rows + kPlanThreads - 1) / kPlanThreads);
     hipLaunchKernelGGL(small ? k_paged_plan<kPlanSmall> : k_paged_plan<kPlanMost>, dim3(groups), dim3(kPlanThreads), 0, s, a);
-    if (!a.one)
+    if (!a.end)
         hipLaunchKernelGGL(small ? k_paged_plan_end<kPlanSmall> : k_paged_plan_end<kPlanMost>, dim3(1), dim3(kPlanThreads),
                            0, s, a);
     PTMI_HIP(hipGetLastError());

@@ -94,6 +94,10 @@ def test_plan_many_rows():
         table[i, :n] = ids[at:at + n]
         at += n
     assert check_plan(past, fresh, ids[at:].tolist(), need + 9, page, table, 45000) == 0
+    assert check_plan(past, fresh, ids[at:].tolist(), need + 9, page, table, 45000, alias=True) == 0
+    for alias in (False, True):                                # refused by all workgroups alike
+        assert check_plan(past, fresh, ids[at:].tolist(), need + 9, page, table, 42000, alias) == 4
+        assert check_plan(past, fresh, ids[at:-12].tolist(), need + 9, page, table, 45000, alias) == 1
 
 
 @pytest.mark.parametrize("what", ["pool", "width", "rows", "past", "fresh", "overflow", "huge", "count", "back"])
